@@ -233,6 +233,120 @@ size_t kq_qmat_bytes(const kq_qmat* a);
 #define KQ_NOALLOC_MAX_ROWS 262144
 int kq_qmat_argmax_noalloc(kq_qmat* a, const float* x_dev, int32_t* idx_dev, void* stream);
 
+/* ------------------------------------------------------------------ serving operators on device tensors
+ * These entry points have no counterpart in the reference; they are additions of this library. They
+ * work on the caller's own device tensors, are enqueued on `stream` (0 = legacy default) without
+ * synchronising and allocate nothing. Sizes, strides, types and alignment are checked on the host
+ * (KQ_ERR_ARG, nothing is launched). What only the device can see -- a page id, a position, a length,
+ * a row index out of range -- never reaches memory: the kernels skip it as each operator says and
+ * leave a flag that kq_stream_check reports as KQ_ERR_ARG.
+ *
+ * A paged K/V cache of one attention layer: K and V are arrays of pages of `page` positions each,
+ * element (page, kv head, row, dim) at page * k_page + head * k_head + row * k_row + dim (elements).
+ * Position p of a sequence is row p % page of the page its table row names at p / page, so a page
+ * may be shared by several tables, and pages may hold anything in the rows not yet written. */
+#define KQ_F32  0
+#define KQ_F16  1
+#define KQ_BF16 2
+#define KQ_E4M3 3                       /* 8-bit floats (4 exponent, 3 mantissa bits, largest 448) */
+
+typedef struct {
+  void *k, *v;                          /* device, 16-byte aligned */
+  long long k_page, k_head, k_row;      /* strides in elements, multiples of 16 bytes; dims are dense */
+  long long v_page, v_head, v_row;
+  const float *k_scale, *v_scale;       /* device [n_kv_heads]: a stored element x stands for x * scale; KQ_E4M3 only, or null (1) */
+  int type;                             /* KQ_F16, KQ_BF16 or KQ_E4M3 */
+  int n_pages, page;                    /* page: a power of two, 16 to 1024 */
+  int n_kv_heads, head_dim;             /* head_dim 64, 128 or 256 */
+} kq_page_desc;
+
+typedef struct kq_pages kq_pages;       /* opaque: the description and the attention's scratch */
+/* The tensors stay the caller's. One scratch per handle: attention calls on one handle that overlap in
+ * time (different streams) race; use one handle per stream. NULL on failure, see kq_error. */
+kq_pages* kq_pages_create(const kq_page_desc* d, int device);
+void kq_pages_free(kq_pages* c);
+
+/* Appends n tokens: the key and value rows of token i, [n_kv_heads][head_dim], go to position pos[i]
+ * of the sequence with page-table row seq[i] (null: row i), the keys rotated by that position on the
+ * way, and so are the queries, from q to q_out (which may be q; both null: none). With r = rot and
+ * angles a = (cos, sin)[pos]: x[j], x[j + r/2] (j < r/2) become x[j] cos - x[j + r/2] sin and
+ * x[j + r/2] cos + x[j] sin; dims from r on stay (the pairs of the decode path's rotation). rot 0 (cos,
+ * sin null): no rotation. Arithmetic in 32 bits, one rounding to the stored type (KQ_E4M3: of
+ * x / scale, saturating at 448). Slots of one call must be distinct.
+ * A token with pos[i] < 0 is skipped entirely (a padded batch). Flagged: a table row or a position
+ * past the table, or a page id outside [0, n_pages) (the token's K/V is not stored, its queries are
+ * turned), a position past the rotation table (the token is skipped). */
+typedef struct {
+  const void *k, *v, *q;                /* rows of src_type: token i, head h at i * x_tok + h * x_head, 16-byte aligned */
+  void* q_out;
+  long long k_tok, k_head, v_tok, v_head, q_tok, q_head, o_tok, o_head;
+  const int32_t* table;                 /* [n_seq][max_pages], row stride table_ld */
+  const int32_t* seq;                   /* [n] or null */
+  const int32_t* pos;                   /* [n] */
+  const float *cos_t, *sin_t;           /* [n_pos][rot / 2], row stride rope_ld, 16-byte aligned */
+  long long table_ld, rope_ld;
+  int n, n_heads;                       /* n_heads: query heads (0 without q) */
+  int src_type;                         /* KQ_F32, KQ_F16 or KQ_BF16 */
+  int n_seq, max_pages;
+  int rot, n_pos;                       /* rot: a multiple of 16, at most head_dim */
+} kq_append_args;
+int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream);
+
+/* Attention of one token of each of n sequences over its cached positions t in [0, len[i]) (window > 0:
+ * the last `window` of them): out[i][h] = sum_t softmax_t(scale q[i][h] . K[t][g]) V[t][g], with
+ * g = h / (n_heads / n_kv_heads), sums and softmax in 32 bits. No position: zeros. The splits of a
+ * long sequence are joined in a fixed order, so equal calls give equal bits.
+ * Flagged: a table row out of range (zeros), len[i] past the table (cut there), a page id outside
+ * [0, n_pages) (its positions are left out); len[i] < 0 counts as 0. */
+typedef struct {
+  const void* q;                        /* token i, head h at i * q_tok + h * q_head, 16-byte aligned */
+  void* out;                            /* of the same type */
+  long long q_tok, q_head, o_tok, o_head;
+  const int32_t* table;                 /* [n_seq][max_pages], row stride table_ld */
+  const int32_t* seq;                   /* [n] or null: token i has table row i */
+  const int32_t* len;                   /* [n] */
+  long long table_ld;
+  int n, n_heads, type;                 /* type of q and out: KQ_F32, KQ_F16 or KQ_BF16 */
+  int n_seq, max_pages, window;
+  float scale;
+} kq_attend_args;
+int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream);
+
+/* Rules on the logits of n rows, and their greedy ids. Row i: with its history hist[i][0 .. hist_len[i])
+ * (the prompt is its first prompt_len[i] tokens), an id's count c in the part after the prompt, and
+ * `seen` if it is anywhere in the history, in this order and in 32 bits:
+ *   z = seen ? (z > 0 ? z / repetition[i] : z * repetition[i]) : z
+ *   z = z - (frequency[i] * c + presence[i] * (c > 0 ? 1 : 0))
+ *   z = z + bias of the id (the last entry with this id in the row's list)
+ *   z = -infinity where the row's mask (bit id % 32 of word id / 32) is 0
+ * rounded once to `type`. best[i] = the lowest id of the largest output, -1 if all are -infinity or NaN.
+ * out may be the logits themselves. Every rule may be absent (null). Ids outside [0, vocab) in a
+ * history or a list are ignored (padding). mask_row[i]: row of the mask array, -1: no mask; null: row i.
+ * Flagged: a mask row out of range (the row then allows nothing). */
+#define KQ_RULES_MAX_VOCAB 393216
+typedef struct {
+  const void* logits;                   /* row i at i * in_ld (elements) */
+  void* out;
+  long long in_ld, out_ld;
+  int32_t* best;                        /* [n] or null */
+  const int32_t* hist;                  /* [n][max_hist], row stride hist_ld, or null */
+  const int32_t *hist_len, *prompt_len; /* [n]; prompt_len null: 0 */
+  long long hist_ld;
+  const float *repetition, *frequency, *presence;   /* [n] or null (1, 0, 0) */
+  const int32_t* bias_id;               /* [n][n_bias], row stride bias_ld (both arrays), or null */
+  const float* bias;
+  long long bias_ld;
+  const uint32_t* mask;                 /* [n_masks] rows of at least ceil(vocab / 32) words, stride mask_ld, or null */
+  const int32_t* mask_row;              /* [n] or null */
+  long long mask_ld;
+  int n, vocab, type;                   /* KQ_F32, KQ_F16 or KQ_BF16 */
+  int max_hist, n_bias, n_masks;
+} kq_rule_args;
+int kq_logit_rules(const kq_rule_args* a, int device, void* stream);
+
+/* Waits for `stream` and reports (and clears) what the operators' kernels flagged on this device. */
+int kq_stream_check(int device, void* stream);
+
 /* ------------------------------------------------------------------ prompt-lookup drafter
  * Replaces NgramDraft (scripts/kindi_q4/kindi/spec.py:801-841): the tokens that followed the
  * latest earlier occurrence of the longest matching suffix of the history, suffix lengths

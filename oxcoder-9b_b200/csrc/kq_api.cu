@@ -7,6 +7,7 @@
 // per token. There is no CPU fallback: every entry point fails with KQ_ERR_BACKEND if CUDA does.
 #include "../../include/kq.h"
 #include "kq_common.cuh"
+#include "kq_host.h"
 #include "kq_qformat.cuh"
 #include "kq_gemv.cuh"
 #include "kq_gemv_mma.cuh"
@@ -129,8 +130,8 @@ static int dev_init(int device) {
     const char* ev = std::getenv("KQ_TMV");   // opt-in while it is validated: 1 = the tensor-core GEMV
     d.tmv_smem = (ev && std::atoi(ev) == 1) ? budget : 0;
   }
-  CU(cudaMalloc(&d.err, sizeof(int)));
-  CU(cudaMemset(d.err, 0, sizeof(int)));
+  CU(cudaMalloc(&d.err, 2 * sizeof(int)));   // [0] matrix-hook calls, [1] serving operators (kq_serve.cu)
+  CU(cudaMemset(d.err, 0, 2 * sizeof(int)));
   d.init = true;
   return KQ_OK;
 }
@@ -2559,6 +2560,16 @@ static int dev_err_check(int device) {
     cudaMemset(g_dev[device].err, 0, sizeof(int));
     return set_err(KQ_ERR_TIMEOUT, "a bounded device wait gave up");
   }
+  return KQ_OK;
+}
+
+int kqh_error(int code, const std::string& msg) { return set_err(code, msg); }
+int kqh_device(int device, KqhDevice* out) {
+  const int rc = dev_init(device);
+  if (rc) return rc;
+  CU(cudaSetDevice(device));
+  out->nsm = g_dev[device].nsm;
+  out->err = g_dev[device].err + 1;
   return KQ_OK;
 }
 

@@ -18,6 +18,9 @@ enum : int {
   KQ_DEV_ERR_BAD_TOKEN = 8,     // a token id outside [0, vocab) reached a kernel
   KQ_DEV_ERR_BAD_POS = 16,      // a position outside [0, ctx) reached a kernel
   KQ_DEV_ERR_GRID = 32,         // a software grid-barrier wait gave up
+  KQ_DEV_ERR_BAD_PAGE = 64,     // a page id outside [0, n_pages) in a page table
+  KQ_DEV_ERR_BAD_LEN = 128,     // a length past its table or array
+  KQ_DEV_ERR_BAD_ROW = 256,     // a row index (page table, mask) out of range
 };
 
 // Polls of mbarrier.try_wait before giving up. Each poll may suspend the thread for a

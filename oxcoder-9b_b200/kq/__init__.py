@@ -100,6 +100,12 @@ SIGNATURES = {
     "kq_draft_logits": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_int)]),
     "kq_draft_upload": (C.c_int, [C.c_void_p, PF, C.c_int]),
     "kq_commit": (C.c_int, [C.c_void_p, PI32, C.c_int, C.c_int]),
+    "kq_pages_create": (C.c_void_p, [C.c_char_p, C.c_int]),
+    "kq_pages_free": (None, [C.c_void_p]),
+    "kq_page_append": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p]),
+    "kq_page_attend": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p]),
+    "kq_logit_rules": (C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
+    "kq_stream_check": (C.c_int, [C.c_int, C.c_void_p]),
     "kq_ngram_create": (C.c_void_p, [C.c_int, C.c_int]),
     "kq_ngram_free": (None, [C.c_void_p]),
     "kq_ngram_reset": (C.c_int, [C.c_void_p, PI32, C.c_int]),
@@ -535,3 +541,6 @@ def make_engine(pack=None, ctx=4096, clusters=None, log=print, device=0, seed=0,
     if ctx is not None:
         overrides["ctx"] = ctx
     return Engine(pack, device=device, seed=seed, **overrides)
+
+
+from .serve import PagedCache, check_stream, logit_rules  # noqa: E402,F401

@@ -1,0 +1,240 @@
+"""kq.serve -- the serving operators on device tensors (include/kq.h, "serving operators"):
+
+    cache = kq.PagedCache(k, v)                     # pages of one attention layer, the caller's tensors
+    cache.append(k_new, v_new, table, pos, rope=(cos, sin), q=q, q_out=q)
+    cache.attend(q, table, lens, out)
+    kq.logit_rules(logits, out, best=ids, hist=..., mask=...)
+    kq.check_stream()                               # waits, raises what the kernels flagged
+
+Tensors are any objects with PyTorch's tensor interface (data_ptr, shape, stride, dtype, get_device);
+this module does not import it. Calls are enqueued on `stream` (a CUDA stream handle, 0 = legacy
+default) and neither wait nor allocate. Wrong types, shapes, strides or devices raise ValueError
+before anything is launched."""
+import ctypes as C
+import struct
+
+F32, F16, BF16, E4M3, I32 = 0, 1, 2, 3, 4
+_NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "float8_e4m3fn": E4M3, "int32": I32, "uint32": I32}
+_types = {}     # dtype object -> code
+
+_APPEND = struct.Struct("4P8q3P2P2q7i4x")
+_ATTEND = struct.Struct("2P4q3Pq6if4x")
+_RULES = struct.Struct("2P2qP3Pq3P2Pq2Pq6i")
+
+
+def _bind():
+    from . import check, last_error, lib
+    return lib(), check, last_error
+
+
+def _type(t):
+    c = _types.get(t.dtype)
+    if c is None:
+        c = _types[t.dtype] = _NAMES.get(str(t.dtype).rpartition(".")[2], -1)
+    return c
+
+
+def _expect(t, what, kind, shape, device):
+    """Pointer of a tensor of this type code (or codes), shape and device whose last dim is dense."""
+    if t.get_device() != device:
+        raise ValueError("%s is not on device %d" % (what, device))
+    if _type(t) != kind:
+        raise ValueError("%s has an unsupported or another type: %s" % (what, t.dtype))
+    if tuple(t.shape) != shape:
+        raise ValueError("%s must have the shape %s, not %s" % (what, shape, tuple(t.shape)))
+    if t.stride(-1) != 1 and shape[-1] > 1:
+        raise ValueError("the last dimension of %s must be dense" % what)
+    return t.data_ptr()
+
+
+class PagedCache(object):
+    """K and V pages of one attention layer: tensors [n_pages, n_kv_heads, page, head_dim] of fp16, bf16
+    or e4m3 (any strides with dense rows on 16-byte boundaries: a transposed view of
+    [n_pages, page, n_kv_heads, head_dim] will do). k_scale, v_scale (e4m3 only): fp32 [n_kv_heads], a stored
+    x stands for x * scale. The tensors stay the caller's and are kept alive by this object. Calls on
+    one cache that overlap in time on different streams race: use one PagedCache for each stream."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        lib, check, error = _bind()
+        self.h = None
+        self._check = check
+        self._free = lib.kq_pages_free
+        if len(k.shape) != 4:
+            raise ValueError("K pages must be [n_pages, n_kv_heads, page, head_dim]")
+        self.device = k.get_device()
+        if self.device < 0:
+            raise ValueError("the pages must be on a GPU")
+        self.n_pages, self.n_kv, self.page, self.hd = shape = tuple(k.shape)
+        self.type = _type(k)
+        if self.type not in (F16, BF16, E4M3):
+            raise ValueError("pages are float16, bfloat16 or float8_e4m3fn, not %s" % k.dtype)
+        kp = _expect(k, "k", self.type, shape, self.device)
+        vp = _expect(v, "v", self.type, shape, self.device)
+        ks = None if k_scale is None else _expect(k_scale, "k_scale", F32, (self.n_kv,), self.device)
+        vs = None if v_scale is None else _expect(v_scale, "v_scale", F32, (self.n_kv,), self.device)
+        self.tensors = (k, v, k_scale, v_scale)
+        d = struct.pack("2P6q2P5i4x", kp, vp, *k.stride()[:3], *v.stride()[:3], ks or 0, vs or 0, self.type, self.n_pages,
+                        self.page, self.n_kv, self.hd)
+        h = lib.kq_pages_create(d, self.device)
+        if not h:
+            raise (MemoryError if "alloc" in error() else ValueError)(error())
+        self.h = C.c_void_p(h)
+        self._append, self._attend = lib.kq_page_append, lib.kq_page_attend
+
+    def close(self):
+        if self.h:
+            self._free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _table(self, table, seq, n):
+        if len(table.shape) != 2:
+            raise ValueError("the page table must be [sequences, pages]")
+        n_seq, wide = table.shape
+        t = _expect(table, "table", I32, (n_seq, wide), self.device)
+        s = 0
+        if seq is not None:
+            s = _expect(seq, "seq", I32, (n,), self.device)
+        elif n > n_seq:
+            raise ValueError("more tokens than page-table rows: give seq")
+        return t, s, table.stride(0) if n_seq > 1 else wide, n_seq, wide
+
+    def append(self, k, v, table, pos, seq=None, rope=None, q=None, q_out=None, stream=0):
+        """K/V rows k, v [n, n_kv_heads, head_dim] (fp32, fp16 or bf16) to positions pos [n] of the sequences whose
+        page-table rows are seq [n] (None: row i for token i); table [sequences, pages] int32. rope: (cos, sin)
+        fp32 [positions, rot / 2]: the keys are rotated on the way, and so are the queries q [n, heads,
+        head_dim] into q_out (may be q). pos < 0 skips a token. Slots of one call must be distinct."""
+        if not self.h:
+            raise ValueError("the cache is closed")
+        n, dev, hd = k.shape[0], self.device, self.hd
+        kind = _type(k)
+        shape = (n, self.n_kv, hd)
+        kp, vp = _expect(k, "k", kind, shape, dev), _expect(v, "v", kind, shape, dev)
+        tp, sp, ld, n_seq, wide = self._table(table, seq, n)
+        pp = _expect(pos, "pos", I32, (n,), dev)
+        cp = np_ = rot = rl = n_pos = 0
+        if rope is not None:
+            cos, sin = rope
+            n_pos, half = cos.shape
+            cp, np_ = _expect(cos, "cos", F32, (n_pos, half), dev), _expect(sin, "sin", F32, (n_pos, half), dev)
+            rl, rot = cos.stride(0) if n_pos > 1 else half, 2 * half
+            if n_pos > 1 and sin.stride(0) != rl:
+                raise ValueError("cos and sin must have the same strides")
+        qp = op = q0 = q1 = o0 = o1 = heads = 0
+        if q is not None:
+            heads = q.shape[1]
+            if q_out is None:
+                raise ValueError("queries need q_out")
+            shape = (n, heads, hd)
+            qp, op = _expect(q, "q", kind, shape, dev), _expect(q_out, "q_out", kind, shape, dev)
+            q0, q1, _ = q.stride()
+            o0, o1, _ = q_out.stride()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if not n:
+            return
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        rc = self._append(self.h, _APPEND.pack(kp, vp, qp, op, k0, k1, v0, v1, q0, q1, o0, o1, tp, sp, pp, cp, np_, ld, rl, n,
+                                               heads, kind, n_seq, wide, rot, n_pos), stream)
+        if rc:
+            self._check(rc)
+
+    def attend(self, q, table, lens, out, seq=None, window=0, scale=None, stream=0):
+        """out[i][h] = softmax(scale q[i][h] . K) V over positions [0, lens[i]) of the sequence with page-table row
+        seq[i] (None: row i); window > 0: over its last `window` positions. q, out [n, heads, head_dim] of one
+        type (fp32, fp16, bf16), scale: 1 / sqrt(head_dim) by default. A row without positions gives zeros."""
+        if not self.h:
+            raise ValueError("the cache is closed")
+        n, heads, hd = shape = tuple(q.shape)
+        dev, kind = self.device, _type(q)
+        if hd != self.hd:
+            raise ValueError("q has head_dim %d, the cache %d" % (hd, self.hd))
+        qp, op = _expect(q, "q", kind, shape, dev), _expect(out, "out", kind, shape, dev)
+        tp, sp, ld, n_seq, wide = self._table(table, seq, n)
+        lp = _expect(lens, "lens", I32, (n,), dev)
+        if not n:
+            return out
+        q0, q1, _ = q.stride()
+        o0, o1, _ = out.stride()
+        rc = self._attend(self.h, _ATTEND.pack(qp, op, q0, q1, o0, o1, tp, sp, lp, ld, n, heads, kind, n_seq, wide, window,
+                                               hd ** -0.5 if scale is None else scale), stream)
+        if rc:
+            self._check(rc)
+        return out
+
+
+def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=None, repetition=None, frequency=None,
+                presence=None, bias_ids=None, bias=None, mask=None, mask_row=None, stream=0):
+    """Penalties for repeated tokens, biases and grammar masks on logits [n, vocab] (fp32, fp16, bf16), into out
+    (may be logits); best [n] int32: the greedy ids (-1 where nothing is allowed). hist [n, most] int32 with
+    hist_len [n] tokens in use, of which prompt_len [n] (None: 0) are the prompt; repetition, frequency, presence:
+    fp32 [n]; bias_ids int32 and bias fp32 [n, entries] (ids outside the vocabulary are padding; the last entry
+    of an id stands); mask int32 or uint32 [masks, >= ceil(vocab / 32)], bit id % 32 of word id / 32 set: allowed;
+    mask_row [n]: a mask for each row, -1 for none (None: mask i for row i)."""
+    lib, check, _ = _bind()
+    n, vocab = shape = tuple(logits.shape)
+    dev, kind = logits.get_device(), _type(logits)
+    if dev < 0:
+        raise ValueError("the logits must be on a GPU")
+    ip, op = _expect(logits, "logits", kind, shape, dev), _expect(out, "out", kind, shape, dev)
+    row = (n,)
+    bp = 0 if best is None else _expect(best, "best", I32, row, dev)
+    hp = hl = pl = hld = most = 0
+    if hist is not None:
+        if hist_len is None:
+            raise ValueError("hist needs hist_len")
+        most = hist.shape[1]
+        hp, hl = _expect(hist, "hist", I32, (n, most), dev), _expect(hist_len, "hist_len", I32, row, dev)
+        hld = hist.stride(0) if n > 1 else most
+        if not most:
+            hp = hl = 0
+    elif hist_len is not None or prompt_len is not None:
+        raise ValueError("history lengths without a history")
+    if prompt_len is not None:
+        pl = _expect(prompt_len, "prompt_len", I32, row, dev) if hp else 0
+    rp = 0 if repetition is None else _expect(repetition, "repetition", F32, row, dev)
+    fp = 0 if frequency is None else _expect(frequency, "frequency", F32, row, dev)
+    sp = 0 if presence is None else _expect(presence, "presence", F32, row, dev)
+    ap = dp = bld = entries = 0
+    if bias_ids is not None and bias is not None:
+        entries = bias_ids.shape[1]
+        ap, dp = _expect(bias_ids, "bias_ids", I32, (n, entries), dev), _expect(bias, "bias", F32, (n, entries), dev)
+        bld = bias.stride(0) if n > 1 else entries
+        if n > 1 and bias_ids.stride(0) != bld:
+            raise ValueError("bias_ids and bias must have the same strides")
+        if not entries:
+            ap = dp = 0
+    elif bias_ids is not None or bias is not None:
+        raise ValueError("bias_ids and bias go together")
+    mp = mr = mld = masks = 0
+    if mask is not None:
+        masks, words = mask.shape
+        mp = _expect(mask, "mask", I32, (masks, words), dev)
+        mld = mask.stride(0) if masks > 1 else words
+        if words < (vocab + 31) // 32:
+            raise ValueError("the masks have too few words")
+        if mask_row is not None:
+            mr = _expect(mask_row, "mask_row", I32, row, dev)
+    elif mask_row is not None:
+        raise ValueError("mask_row without masks")
+    if not n:
+        return out
+    rc = lib.kq_logit_rules(_RULES.pack(ip, op, logits.stride(0) if n > 1 else vocab, out.stride(0) if n > 1 else vocab, bp,
+                                        hp, hl, pl, hld, rp, fp, sp, ap, dp, bld, mp, mr, mld, n, vocab, kind, most, entries,
+                                        masks), dev, stream)
+    if rc:
+        check(rc)
+    return out
+
+
+def check_stream(device=0, stream=0):
+    """Waits for the stream and raises ValueError if an operator's kernel met a page id, position, length or row
+    index out of range since the last check on this device (such entries are skipped, never read)."""
+    lib, check, _ = _bind()
+    check(lib.kq_stream_check(device, stream))
