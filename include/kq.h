@@ -295,7 +295,8 @@ int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream);
 /* Attention of one token of each of n sequences over its cached positions t in [0, len[i]) (window > 0:
  * the last `window` of them): out[i][h] = sum_t softmax_t(scale q[i][h] . K[t][g]) V[t][g], with
  * g = h / (n_heads / n_kv_heads), sums and softmax in 32 bits. No position: zeros. The splits of a
- * long sequence are joined in a fixed order, so equal calls give equal bits.
+ * long sequence are joined in a fixed order, so equal calls give equal bits. Positions outside the
+ * range are never read; inside it, an infinite V gives NaN (the weights are multiplied in two parts).
  * Flagged: a table row out of range (zeros), len[i] past the table (cut there), a page id outside
  * [0, n_pages) (its positions are left out); len[i] < 0 counts as 0. */
 typedef struct {

@@ -131,57 +131,481 @@ __device__ __forceinline__ KeyRange pg_keys(const AttendParams& P, int i, bool r
   return R;
 }
 
-// Grid (token, query head), 4 warps: a warp takes every fourth key, a lane HD / 32 dims; online
-// softmax per warp, the warps joined in order.
-template <int HD>
-__global__ void __launch_bounds__(128) k_page_attend(const __grid_constant__ AttendParams P) {
-  constexpr int D = HD / 32;
-  const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = h / (P.n_heads / P.n_kv);
-  __shared__ float s_m[4], s_l[4], s_o[4][HD];
-  const KeyRange R = pg_keys(P, i, threadIdx.x == 0);
-  float q[D], o[D], m = -INFINITY, l = 0.f;
-  const float scale = P.scale * (P.ks ? P.ks[g] : 1.f);
+// ---- matrix-instruction fragments. S^T = K Q^T and O^T = V^T P^T on m16n8k16 (fp16 or bf16 operands,
+// fp32 accumulation): the keys (then the dims) are the 16 rows and 8 query heads of one K/V head the
+// columns, so a group of up to 8 heads wastes no rows, and a thread keeps the two heads 2 t4,
+// 2 t4 + 1 in every accumulator (grp = lane / 4, t4 = lane % 4).
+template <bool BF>
+__device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t pa_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Two e4m3 bytes (the low half of x) as fp16; exact.
+__device__ __forceinline__ uint32_t pa_e4m3x2(uint32_t x) {
+  uint32_t d;
+  asm volatile("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(d) : "r"(x));
+  return d;
+}
+// N 16-bit terms whose sum is (a, b) to N * 11 (fp16) or N * 8 (bf16) bits, largest first.
+template <bool BF, int N>
+__device__ __forceinline__ void pa_split(float a, float b, uint32_t (&t)[N]) {
 #pragma unroll
-  for (int d = 0; d < D; ++d) {
-    q[d] = pg_load(P.q, P.type, i * P.q_tok + h * P.q_head + D * lane + d);
-    o[d] = 0.f;
-  }
-  for (int t = R.first + warp; t < R.last; t += 4) {
-    const int page = P.T.table[R.row * P.T.ld + (t >> P.T.page_shift)], row = t & ((1 << P.T.page_shift) - 1);
-    if (page < 0 || page >= P.T.n_pages) {
-      if (lane == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
-      continue;
+  for (int i = 0; i < N; ++i) {
+    float x, y;
+    if (BF) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+      t[i] = *reinterpret_cast<const uint32_t*>(&h);
+      x = __bfloat162float(h.x);
+      y = __bfloat162float(h.y);
+    } else {
+      const __half2 h = __floats2half2_rn(a, b);
+      t[i] = *reinterpret_cast<const uint32_t*>(&h);
+      x = __half2float(h.x);
+      y = __half2float(h.y);
     }
-    const long long k0 = page * P.kp + g * P.kh + row * P.kr, v0 = page * P.vp + g * P.vh + row * P.vr;
-    float s = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) s = __fmaf_rn(q[d], pg_load(P.kc, P.cache_type, k0 + D * lane + d), s);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    s *= scale;
-    const float mn = fmaxf(m, s), u = mn == -INFINITY ? 0.f : mn, f = expf(m - u), p = expf(s - u);
-    m = mn;
-    l = __fmaf_rn(l, f, p);
-#pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = __fmaf_rn(o[d], f, p * pg_load(P.vc, P.cache_type, v0 + D * lane + d));
+    if (i + 1 < N) {
+      a = __fsub_rn(a, x);
+      b = __fsub_rn(b, y);
+    }
   }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+}
+
+constexpr int PA_WARPS = 4;
+constexpr int PA_SUB = 16;                     // keys of one warp's step: within one page, whose size is a multiple of 16
+constexpr int PA_TILE = PA_WARPS * PA_SUB;     // the unit the work is divided in
+constexpr int PA_MAX_CTAS = 148 * 2;           // CTAs of one launch, and partial slots (two each) of the scratch
+constexpr int PA_MAX_HEADS = 16;               // query heads of one K/V head a CTA takes at once
+
+template <int CT, int HD, int NT, bool PREC>
+struct PaShape {
+  static constexpr bool BF = CT == PG_BF16;
+  static constexpr int ES = CT == PG_E4M3 ? 1 : 2;
+  static constexpr int ROW = HD * ES, LD = ROW + 16;           // odd multiples of 16 bytes: conflict-free ldmatrix rows
+  static constexpr int STAGE = 2 * PA_SUB * LD;                // K and V rows of one step of a warp
+  static constexpr int FIT = 104 * 1024 / (PA_WARPS * STAGE);
+  static constexpr int STAGES = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;   // two CTAs per SM where three stages leave the room
+  static constexpr int KS = HD / 16;
+  static constexpr int NQ = PREC ? (BF ? 3 : 2) : 1;           // terms of a query element
+  static constexpr int NP = PREC ? (BF ? 3 : 2) : 2;           // terms of a softmax weight
+  static constexpr bool QREG = KS * NQ * NT * 2 <= 64;         // query fragments in registers, else in shared memory
+  static constexpr int QBYTES = QREG ? 0 : KS * NQ * NT * 256;
+  static constexpr int HEADS = 8 * NT;
+  static constexpr int MLD = HD + 4;                           // row of the warps' exchange: o, m, l
+  static constexpr int RING = PA_WARPS * STAGES * STAGE;
+  static constexpr int XCHG = PA_WARPS * HEADS * MLD * 4;
+  static constexpr int SMEM = (RING > XCHG ? RING : XCHG) + QBYTES;
+};
+constexpr int PA_PLD = 256 + 4;                // floats of a scratch row (the widest head_dim)
+
+struct AttendScratch {
+  float* part;      // [2 * PA_MAX_CTAS][PA_MAX_HEADS][PA_PLD]: o, m, l of a CTA's first (0) and last (1) segment
+  int* ticket;      // [PA_MAX_CTAS], zero between launches
+};
+
+// The tiles of all (sequence, virtual head, 64-key tile) triples, in this order, are cut into equal
+// runs, one per CTA, wherever sequences end: CTAs finish together whatever the lengths are. A CTA
+// walks its run segment by segment (one sequence and head at a time). A segment that is a whole
+// (sequence, head) is written out; otherwise its (o, m, l) goes to the scratch and the last CTA of
+// the chain to arrive joins the chain's partials in CTA order, so the sums' order is fixed.
+template <int CT, int HD, int NT, bool PREC>
+__global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
+  using S = PaShape<CT, HD, NT, PREC>;
+  constexpr bool BF = S::BF, E8 = CT == PG_E4M3;
+  constexpr int KS = S::KS, NQ = S::NQ, NP = S::NP;
+  constexpr float PSCALE = BF ? 1.f : 16384.f;   // fp16 weights use 2^14 .. 2^-24: 38 bits below the largest
+  extern __shared__ __align__(128) uint8_t pa_smem[];
+  __shared__ long long s_start, s_total;
+  __shared__ long long s_scan[PA_WARPS];
+  __shared__ int s_seq, s_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, t4 = lane & 3;
+  const int G = P.n_heads / P.n_kv, HT = (G + S::HEADS - 1) / S::HEADS, H = P.n_kv * HT;
+
+  auto tiles_of = [&](int i, KeyRange& R) {
+    R = pg_keys(P, i, false);
+    return R.last > R.first ? (R.last - (R.first & ~(PA_SUB - 1)) + PA_TILE - 1) / PA_TILE : 0;
+  };
+  // ---- where this CTA's run begins: a scan of the sequences' tiles, consecutive ones per thread
+  const int per = (P.n + PA_WARPS * 32 - 1) / (PA_WARPS * 32), i0 = min(P.n, tid * per), i1 = min(P.n, i0 + per);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) {
+    if (blockIdx.x == 0) pg_keys(P, i, true);
+    KeyRange R;
+    mine += tiles_of(i, R);
+  }
+  long long incl = mine;
 #pragma unroll
-  for (int d = 0; d < D; ++d) s_o[warp][D * lane + d] = o[d];
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += v;
+  }
+  if (lane == 31) s_scan[warp] = incl;
   __syncthreads();
-  float M = -INFINITY, L = 0.f, w[4];
-  for (int x = 0; x < 4; ++x) M = fmaxf(M, s_m[x]);
-  for (int x = 0; x < 4; ++x) {
-    w[x] = s_m[x] == -INFINITY && !(s_l[x] != 0.f) ? 0.f : expf(s_m[x] - (M == -INFINITY ? 0.f : M));
-    L = __fmaf_rn(w[x], s_l[x], L);
+  long long before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
   }
-  const float vs = P.vs ? P.vs[g] : 1.f;
-  for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-    float v = 0.f;
-    for (int x = 0; x < 4; ++x)
-      if (w[x] != 0.f) v = __fmaf_rn(w[x], s_o[x][d], v);
-    pg_store(P.out, P.type, i * P.o_tok + h * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(v, L) * vs);
+  total *= H;
+  const long long run = (total + gridDim.x - 1) / gridDim.x;
+  const long long begin = min(total, blockIdx.x * run), end = min(total, begin + run);
+  if (begin < end && before * H <= begin && begin < (before + mine) * H) {
+    long long b = before;
+    for (int i = i0; i < i1; ++i) {
+      KeyRange R;
+      const int u = tiles_of(i, R);
+      if (begin < (b + u) * H) {
+        s_seq = i;
+        s_start = b * H;
+        break;
+      }
+      b += u;
+    }
+  }
+  if (tid == 0) s_total = total;
+  // rows without a key: zeros
+  for (int i = blockIdx.x; i < P.n; i += gridDim.x) {
+    KeyRange R;
+    if (tiles_of(i, R)) continue;
+    for (int e = tid; e < P.n_heads * HD; e += PA_WARPS * 32) pg_store(P.out, P.type, i * P.o_tok + (e / HD) * P.o_head + e % HD, 0.f);
+  }
+  __syncthreads();
+  if (begin >= end) return;
+
+  const uint32_t ring = smem_u32(pa_smem) + warp * S::STAGES * S::STAGE;
+  uint2* qs = reinterpret_cast<uint2*>(pa_smem + (S::SMEM - S::QBYTES));
+  float* xo = reinterpret_cast<float*>(pa_smem);
+  // this lane's part of a step's rows: 16-byte chunks lane, lane + 32, .. of the 16 rows
+  constexpr int CH = S::ROW / 16, NCP = S::ROW / 32;
+  const int lr = lane / CH, lc = lane % CH;            // CH <= 32: row and chunk of the first one
+  constexpr int RSTEP = 32 / CH;                       // rows between a lane's chunks
+  const int mi = lane >> 3, ml = lane & 7;
+  const uint32_t k_off = (uint32_t)(((mi & 1) * 8 + ml) * S::LD + (mi >> 1) * 16);
+  const uint32_t v_off = (uint32_t)(E8 ? ((mi & 1) * 8 + ml) * S::LD + (mi >> 1) * 16 : ((mi >> 1) * 8 + ml) * S::LD + (mi & 1) * 16) +
+                         PA_SUB * S::LD;
+
+  int seq = s_seq;
+  KeyRange R;
+  int tiles = tiles_of(seq, R);
+  long long seg0 = s_start, left = end - begin;        // first tile of (seq, head 0)
+  long long at = begin - seg0;
+  int head = (int)(at / tiles), tile = (int)(at % tiles);
+  while (left > 0) {
+    // ---- one segment: tiles [tile, tile_end) of (seq, head)
+    const int tile_end = (int)min((long long)tiles, tile + left);
+    const int kv = head / HT, h0 = kv * G + (head % HT) * S::HEADS, nh = min(S::HEADS, (kv + 1) * G - h0);
+    const int base = R.first & ~(PA_SUB - 1);
+    const int k_begin = base + tile * PA_TILE + warp * PA_SUB, k_end = min(R.last, base + tile_end * PA_TILE);
+    const int* pt = P.T.table + R.row * P.T.ld;
+    const char* kg = reinterpret_cast<const char*>(P.kc) + kv * P.kh * S::ES;
+    const char* vg = reinterpret_cast<const char*>(P.vc) + kv * P.vh * S::ES;
+    uint32_t pages_ok = 0;                             // one bit per ring slot: its page exists
+    auto load = [&](int key, int slot) {
+      if (key >= k_end) return;
+      const int page = __ldg(pt + (key >> P.T.page_shift));
+      const bool ok = page >= 0 && page < P.T.n_pages;
+      pages_ok = (pages_ok & ~(1u << slot)) | ((uint32_t)ok << slot);
+      if (!ok && lane == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
+      const long long row = (key & ((1 << P.T.page_shift) - 1)) + lr;
+      const char* ks = kg + (ok ? (page * P.kp + row * P.kr) * S::ES + lc * 16 : 0);
+      const char* vs = vg + (ok ? (page * P.vp + row * P.vr) * S::ES + lc * 16 : 0);
+      const uint32_t d = ring + slot * S::STAGE + lr * S::LD + lc * 16;
+#pragma unroll
+      for (int c = 0; c < NCP; ++c) {
+        const int t = key + lr + c * RSTEP;
+        const bool in = ok && t >= R.first && t < R.last;   // rows outside are not read: they may hold anything
+        pa_cp16(d + c * RSTEP * S::LD, in ? ks + c * RSTEP * P.kr * S::ES : kg, in ? 16u : 0u);
+        pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, in ? vs + c * RSTEP * P.vr * S::ES : vg, in ? 16u : 0u);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < S::STAGES - 1; ++s) {
+      load(k_begin + s * PA_TILE, s);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // ---- query fragments (column grp of each 8 heads), scaled to [2^9, 2^10) by a power of two
+    uint32_t qf[S::QREG ? NQ : 1][S::QREG ? NT : 1][S::QREG ? KS : 1][2];
+    float sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int hh = nt * 8 + grp;
+      const long long qo = seq * P.q_tok + (h0 + min(hh, nh - 1)) * P.q_head;
+      float mx = 0.f;
+      for (int d = 2 * t4; d < HD; d += 8) {
+        const float a = pg_load(P.q, P.type, qo + d), b = pg_load(P.q, P.type, qo + d + 1);
+        mx = fmaxf(mx, fmaxf(fabsf(a), fabsf(b)));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      int e = 0;
+      if (mx > 0.f && mx < INFINITY) e = max(-100, (int)((__float_as_uint(mx) >> 23) & 255u) - 127);
+      const float up = hh < nh ? __uint_as_float((uint32_t)(127 + 9 - e) << 23) : 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (!S::QREG && (ks & 3) != warp) continue;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // the dims of k indices 2 t4, 2 t4 + 1 (+ 8): 8-bit K fragments hold dims 4 t4 .. 4 t4 + 3
+          const int d = 16 * ks + (E8 ? 4 * t4 + 2 * half : 2 * t4 + 8 * half);
+          uint32_t t[NQ];
+          const float a = hh < nh ? pg_load(P.q, P.type, qo + d) * up : 0.f;
+          const float b = hh < nh ? pg_load(P.q, P.type, qo + d + 1) * up : 0.f;
+          pa_split<BF, NQ>(a, b, t);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) {
+            if (S::QREG) qf[j][nt][ks][half] = t[j];
+            else reinterpret_cast<uint32_t*>(qs + ((j * NT + nt) * KS + ks) * 32 + lane)[half] = t[j];
+          }
+        }
+      }
+      const float f = P.scale * 1.4426950408889634f * (P.ks ? P.ks[kv] : 1.f);
+      const int ea = __shfl_sync(0xffffffffu, e, 8 * t4), eb = __shfl_sync(0xffffffffu, e, 8 * t4 + 4);
+      sc[nt][0] = f * __uint_as_float((uint32_t)(127 - 9 + ea) << 23);
+      sc[nt][1] = f * __uint_as_float((uint32_t)(127 - 9 + eb) << 23);
+    }
+    if (!S::QREG) __syncthreads();
+
+    float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < KS; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
+    }
+    int slot = 0, fill = S::STAGES - 1;
+    for (int key = k_begin; key < k_end; key += PA_TILE) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+      __syncwarp();
+      const bool ok = (pages_ok >> slot) & 1u;
+      const uint32_t kb = ring + slot * S::STAGE + k_off, vb = ring + slot * S::STAGE + v_off;
+      load(key + (S::STAGES - 1) * PA_TILE, fill);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      fill = slot;
+      slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+      // ---- scores: the terms of the queries in accumulators of their own, smallest added first
+      float s[NQ][NT][4];
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[j][nt][0] = s[j][nt][1] = s[j][nt][2] = s[j][nt][3] = 0.f;
+      auto score = [&](int ks, const uint32_t (&a)[4]) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if (S::QREG) pa_mma<BF>(s[j][nt], a, qf[j][nt][ks][0], qf[j][nt][ks][1]);
+            else {
+              const uint2 b = qs[((j * NT + nt) * KS + ks) * 32 + lane];
+              pa_mma<BF>(s[j][nt], a, b.x, b.y);
+            }
+          }
+      };
+      if (E8) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          uint32_t r[4];
+          pa_ldsm(kb + ks * 16, r);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t a[4] = {pa_e4m3x2(r[2 * j]), pa_e4m3x2(r[2 * j + 1]), pa_e4m3x2(r[2 * j] >> 16), pa_e4m3x2(r[2 * j + 1] >> 16)};
+            score(ks + j, a);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t a[4];
+          pa_ldsm(kb + ks * 32, a);
+          score(ks, a);
+        }
+      }
+      // ---- online softmax, in powers of two: rows (keys) grp and grp + 8, heads 2 t4 and 2 t4 + 1
+      const bool va = ok && key + grp >= R.first && key + grp < R.last;
+      const bool vb8 = ok && key + grp + 8 >= R.first && key + grp + 8 < R.last;
+      uint32_t pf[NP][NT][2];
+      float f[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // an infinite key makes the leading term's sum infinite and a zero lower term's sum NaN
+          float a = s[NQ - 1][nt][e];
+#pragma unroll
+          for (int j = NQ - 2; j >= 0; --j) a = j > 0 || fabsf(s[0][nt][e]) < INFINITY ? __fadd_rn(a, s[j][nt][e]) : s[0][nt][e];
+          x[e] = (e < 2 ? va : vb8) ? __fmul_rn(a, sc[nt][e & 1]) : -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(x[c], x[c + 2]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[nt][c], mx), u = mn == -INFINITY ? 0.f : mn;
+          f[nt][c] = exp2f(m[nt][c] - u);
+          m[nt][c] = mn;
+          x[c] = exp2f(x[c] - u) * PSCALE;
+          x[c + 2] = exp2f(x[c + 2] - u) * PSCALE;
+          l[nt][c] = __fmaf_rn(l[nt][c], f[nt][c], x[c] + x[c + 2]);
+        }
+        uint32_t ta[NP], tb[NP];
+        pa_split<BF, NP>(x[0], x[1], ta);
+        pa_split<BF, NP>(x[2], x[3], tb);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          pf[j][nt][0] = pa_trans(ta[j]);
+          pf[j][nt][1] = pa_trans(tb[j]);
+        }
+      }
+      // ---- O^T += V^T P^T: a step's product is summed apart and added in fp32 (the matrix units cut
+      // off low bits when they add to a large accumulator; over thousands of steps that would show)
+      auto accumulate = [&](int d, const uint32_t (&a)[4]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = NP - 1; j >= 0; --j) pa_mma<BF>(t, a, pf[j][nt][0], pf[j][nt][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][nt][e] = __fmaf_rn(o[d][nt][e], f[nt][e & 1], t[e]);
+        }
+      };
+      if (E8) {
+        // a 32-bit word of the transposed fragment: dims 2 grp, 2 grp + 1 of keys 2 t4 (low half) and 2 t4 + 1
+#pragma unroll
+        for (int d = 0; d < KS; d += 2) {
+          uint32_t r[4];
+          pa_ldsm_t(vb + d * 16, r);   // keys 0-7, 8-15 of 16 dims, then of the next 16
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t lo = r[2 * j], hi = r[2 * j + 1];
+            const uint32_t a[4] = {pa_e4m3x2(__byte_perm(lo, 0, 0x4420)), pa_e4m3x2(__byte_perm(lo, 0, 0x4431)),
+                                   pa_e4m3x2(__byte_perm(hi, 0, 0x4420)), pa_e4m3x2(__byte_perm(hi, 0, 0x4431))};
+            accumulate(d + j, a);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < KS; ++d) {
+          uint32_t a[4];
+          pa_ldsm_t(vb + d * 32, a);
+          accumulate(d, a);
+        }
+      }
+      __syncwarp();   // the slot may be filled again
+    }
+    // ---- join the warps: (o, m, l) rows through the (drained) ring
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float ls = l[nt][c];
+        ls += __shfl_xor_sync(0xffffffffu, ls, 4);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+        float* row = xo + (warp * S::HEADS + nt * 8 + 2 * t4 + c) * S::MLD;
+        if (grp == 0) {
+          row[HD] = m[nt][c];
+          row[HD + 1] = ls;
+        }
+#pragma unroll
+        for (int d = 0; d < KS; ++d) {
+          row[16 * d + (E8 ? 2 * grp : grp)] = o[d][nt][c];
+          row[16 * d + (E8 ? 2 * grp + 1 : grp + 8)] = o[d][nt][c + 2];
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = tile == 0 && tile_end == tiles;
+    const long long seg_begin = seg0 + (long long)head * tiles;
+    const int slot_id = 2 * blockIdx.x + (tile == 0 ? 1 : 0);
+    float* part = W.part + (size_t)slot_id * PA_MAX_HEADS * PA_PLD;
+    const float vscale = P.vs ? P.vs[kv] : 1.f;
+    for (int e = tid; e < nh * HD; e += PA_WARPS * 32) {
+      const int h = e / HD, d = e % HD;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, xo[(w * S::HEADS + h) * S::MLD + HD]);
+      const float u = M == -INFINITY ? 0.f : M;
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < PA_WARPS; ++w) {
+        const float* row = xo + (w * S::HEADS + h) * S::MLD;
+        const float wt = exp2f(row[HD] - u);
+        L = __fmaf_rn(wt, row[HD + 1], L);
+        O = __fmaf_rn(wt, row[d], O);
+      }
+      if (whole) pg_store(P.out, P.type, seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
+      else {
+        __stcg(part + h * PA_PLD + d, O);
+        if (d == 0) {
+          __stcg(part + h * PA_PLD + HD, M);
+          __stcg(part + h * PA_PLD + HD + 1, L);
+        }
+      }
+    }
+    if (!whole) {
+      const int c0 = (int)(seg_begin / run), c1 = (int)((seg_begin + tiles - 1) / run);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(&W.ticket[c0], 1) == c1 - c0;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (int e = tid; e < nh * HD; e += PA_WARPS * 32) {
+          const int h = e / HD, d = e % HD;
+          float M = -INFINITY;
+          for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(W.part + ((size_t)(2 * c + (c == c0)) * PA_MAX_HEADS + h) * PA_PLD + HD));
+          const float u = M == -INFINITY ? 0.f : M;
+          float L = 0.f, O = 0.f;
+          for (int c = c0; c <= c1; ++c) {
+            const float* row = W.part + ((size_t)(2 * c + (c == c0)) * PA_MAX_HEADS + h) * PA_PLD;
+            const float wt = exp2f(__ldcg(row + HD) - u);
+            L = __fmaf_rn(wt, __ldcg(row + HD + 1), L);
+            O = __fmaf_rn(wt, __ldcg(row + d), O);
+          }
+          pg_store(P.out, P.type, seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
+        }
+        if (tid == 0) W.ticket[c0] = 0;
+      }
+    }
+    __syncthreads();   // the ring and the exchange are free again
+    // ---- next segment
+    left -= tile_end - tile;
+    tile = tile_end;
+    if (tile == tiles) {
+      tile = 0;
+      if (++head == H && left > 0) {
+        head = 0;
+        seg0 += (long long)H * tiles;
+        do tiles = tiles_of(++seq, R);
+        while (tiles == 0);
+      }
+    }
   }
 }
 

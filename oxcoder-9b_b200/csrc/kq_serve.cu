@@ -8,6 +8,7 @@
 #include "kq_rules.cuh"
 
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <new>
 
 using namespace kq;
@@ -24,9 +25,34 @@ using namespace kq;
 
 struct kq_pages {
   kq_page_desc d{};
-  int device = 0, shift = 0, esize = 2;
+  int device = 0, shift = 0;
   KqhDevice dev{};
+  AttendScratch scratch{};
 };
+
+// The attention kernel of a cache type, head size, query heads per CTA (8 or 16) and precision.
+typedef void (*AttendFn)(AttendParams, AttendScratch);
+struct AttendKernel {
+  AttendFn fn;
+  int smem;
+};
+template <int CT, int HD, int NT, bool PREC>
+static AttendKernel attend_entry() {
+  return {k_page_attend<CT, HD, NT, PREC>, PaShape<CT, HD, NT, PREC>::SMEM};
+}
+template <int CT, int HD>
+static AttendKernel attend_of(bool wide, bool prec) {
+  if (wide) return prec ? attend_entry<CT, HD, 2, true>() : attend_entry<CT, HD, 2, false>();
+  return prec ? attend_entry<CT, HD, 1, true>() : attend_entry<CT, HD, 1, false>();
+}
+template <int CT>
+static AttendKernel attend_of(int hd, bool wide, bool prec) {
+  return hd == 64 ? attend_of<CT, 64>(wide, prec) : hd == 128 ? attend_of<CT, 128>(wide, prec) : attend_of<CT, 256>(wide, prec);
+}
+static AttendKernel attend_kernel(int type, int hd, bool wide, bool prec) {
+  return type == KQ_F16 ? attend_of<PG_F16>(hd, wide, prec) : type == KQ_BF16 ? attend_of<PG_BF16>(hd, wide, prec)
+                                                                             : attend_of<PG_E4M3>(hd, wide, prec);
+}
 
 static int type_size(int type) { return type == KQ_F32 ? 4 : type == KQ_E4M3 ? 1 : 2; }
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -60,12 +86,34 @@ extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) {
   c->d = *d;
   c->device = device;
   c->dev = dev;
-  c->esize = type_size(d->type);
   while ((1 << c->shift) < d->page) ++c->shift;
+  const size_t part = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
+  cudaError_t e = cudaMalloc(&c->scratch.part, part + PA_MAX_CTAS * sizeof(int));
+  if (e == cudaSuccess) {
+    c->scratch.ticket = reinterpret_cast<int*>(reinterpret_cast<char*>(c->scratch.part) + part);
+    e = cudaMemset(c->scratch.ticket, 0, PA_MAX_CTAS * sizeof(int));
+  }
+  for (int v = 0; v < 4 && e == cudaSuccess; ++v) {
+    const AttendKernel k = attend_kernel(d->type, d->head_dim, v & 1, v & 2);
+    e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+  }
+  if (e != cudaSuccess) {
+    kqh_error(e == cudaErrorMemoryAllocation ? KQ_ERR_MEMORY : KQ_ERR_BACKEND,
+              std::string("kq_pages_create: scratch allocation or kernel set-up: ") + cudaGetErrorString(e));
+    kq_pages_free(c);
+    return nullptr;
+  }
   return c;
 }
 
-extern "C" void kq_pages_free(kq_pages* c) { delete c; }
+extern "C" void kq_pages_free(kq_pages* c) {
+  if (!c) return;
+  if (c->scratch.part) {
+    cudaSetDevice(c->device);
+    cudaFree(c->scratch.part);
+  }
+  delete c;
+}
 
 static PageTable table_of(const kq_pages* c, const int32_t* table, const int32_t* seq, long long ld, int n_seq, int max_pages) {
   return PageTable{table, seq, ld, n_seq, max_pages, c->d.n_pages, c->shift};
@@ -131,11 +179,17 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream
   P.T = table_of(c, a->table, a->seq, a->table_ld, a->n_seq, a->max_pages);
   P.len = a->len; P.n = a->n; P.n_heads = a->n_heads; P.n_kv = c->d.n_kv_heads; P.type = a->type;
   P.cache_type = c->d.type; P.window = a->window; P.scale = a->scale; P.err = c->dev.err;
-  const dim3 grid((unsigned)a->n, (unsigned)a->n_heads);
-  cudaStream_t s = (cudaStream_t)stream;
-  if (c->d.head_dim == 64) k_page_attend<64><<<grid, 128, 0, s>>>(P);
-  else if (c->d.head_dim == 128) k_page_attend<128><<<grid, 128, 0, s>>>(P);
-  else k_page_attend<256><<<grid, 128, 0, s>>>(P);
+  const int G = a->n_heads / P.n_kv;
+  // fp32 queries want fp32 scores: the cache's 16-bit type in two or three terms; so do fp16 queries
+  // (11 bits) on a bf16 cache (8 bits)
+  const bool prec = a->type == KQ_F32 || (c->d.type == KQ_BF16 && a->type == KQ_F16);
+  const AttendKernel k = attend_kernel(c->d.type, c->d.head_dim, G > 8, prec);
+  const int heads = G > 8 ? 16 : 8;
+  const long long tiles = (((long long)a->max_pages << c->shift) + PA_TILE - 1) / PA_TILE;
+  const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
+  const int per_sm = k.smem > 110 * 1024 ? 1 : 2;
+  const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * per_sm));
+  k.fn<<<grid, PA_WARPS * 32, k.smem, (cudaStream_t)stream>>>(P, c->scratch);
   CU(cudaGetLastError());
   return KQ_OK;
 }
