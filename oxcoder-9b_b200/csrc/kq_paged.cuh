@@ -20,6 +20,12 @@ __device__ __forceinline__ float pg_load(const void* row, int type, long long i)
   if (type == PG_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[i]);
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(reinterpret_cast<const __nv_fp8_storage_t*>(row)[i], __NV_E4M3)));
 }
+// Elements i, i + 1 (i even, the row 4-byte aligned at least) of a row of fp32 or 16-bit elements.
+__device__ __forceinline__ float2 pg_load2(const void* row, int type, long long i) {
+  if (type == PG_F32) return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(row) + i);
+  if (type == PG_F16) return __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const __half*>(row) + i));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(reinterpret_cast<const __nv_bfloat16*>(row) + i));
+}
 // One rounding of an fp32 value to `type` (8-bit floats saturate at 448; NaN stays NaN).
 __device__ __forceinline__ void pg_store(void* row, int type, long long i, float x) {
   if (type == PG_F32) reinterpret_cast<float*>(row)[i] = x;
@@ -353,9 +359,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
       const int hh = nt * 8 + grp;
       const long long qo = seq * P.q_tok + (h0 + min(hh, nh - 1)) * P.q_head;
       float mx = 0.f;
+#pragma unroll
       for (int d = 2 * t4; d < HD; d += 8) {
-        const float a = pg_load(P.q, P.type, qo + d), b = pg_load(P.q, P.type, qo + d + 1);
-        mx = fmaxf(mx, fmaxf(fabsf(a), fabsf(b)));
+        const float2 a = pg_load2(P.q, P.type, qo + d);
+        mx = fmaxf(mx, fmaxf(fabsf(a.x), fabsf(a.y)));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -370,9 +377,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
           // the dims of k indices 2 t4, 2 t4 + 1 (+ 8): 8-bit K fragments hold dims 4 t4 .. 4 t4 + 3
           const int d = 16 * ks + (E8 ? 4 * t4 + 2 * half : 2 * t4 + 8 * half);
           uint32_t t[NQ];
-          const float a = hh < nh ? pg_load(P.q, P.type, qo + d) * up : 0.f;
-          const float b = hh < nh ? pg_load(P.q, P.type, qo + d + 1) * up : 0.f;
-          pa_split<BF, NQ>(a, b, t);
+          const float2 a = hh < nh ? pg_load2(P.q, P.type, qo + d) : make_float2(0.f, 0.f);
+          pa_split<BF, NQ>(a.x * up, a.y * up, t);
 #pragma unroll
           for (int j = 0; j < NQ; ++j) {
             if (S::QREG) qf[j][nt][ks][half] = t[j];
@@ -576,19 +582,69 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
       __syncthreads();
       if (s_last) {
         __threadfence();
-        for (int e = tid; e < nh * HD; e += PA_WARPS * 32) {
-          const int h = e / HD, d = e % HD;
-          float M = -INFINITY;
-          for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(W.part + ((size_t)(2 * c + (c == c0)) * PA_MAX_HEADS + h) * PA_PLD + HD));
-          const float u = M == -INFINITY ? 0.f : M;
-          float L = 0.f, O = 0.f;
-          for (int c = c0; c <= c1; ++c) {
-            const float* row = W.part + ((size_t)(2 * c + (c == c0)) * PA_MAX_HEADS + h) * PA_PLD;
-            const float wt = exp2f(__ldcg(row + HD) - u);
-            L = __fmaf_rn(wt, __ldcg(row + HD + 1), L);
-            O = __fmaf_rn(wt, __ldcg(row + d), O);
+        // weights exp2(m_c - M) of the chain's partials, all requested at once; then float4 columns,
+        // the CTAs' rows split over the thread groups a narrow segment leaves idle
+        const int nc = c1 - c0 + 1;
+        float* sw = xo;                                  // [nh][nc], then L[nh], then the groups' sums
+        float* sl = sw + nh * nc;
+        auto row_of = [&](int c, int h) { return W.part + ((size_t)(2 * (c0 + c) + (c == 0)) * PA_MAX_HEADS + h) * PA_PLD; };
+        for (int h = warp; h < nh; h += PA_WARPS) {
+          float M = -INFINITY, L = 0.f;
+          for (int c = lane; c < nc; c += 32) {
+            const float v = __ldcg(row_of(c, h) + HD);
+            sw[h * nc + c] = v;
+            M = fmaxf(M, v);
           }
-          pg_store(P.out, P.type, seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+          const float u = M == -INFINITY ? 0.f : M;
+          for (int c = lane; c < nc; c += 32) {
+            const float wt = exp2f(sw[h * nc + c] - u);
+            sw[h * nc + c] = wt;
+            L = __fmaf_rn(wt, __ldcg(row_of(c, h) + HD + 1), L);
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, off));
+          if (lane == 0) sl[h] = L;
+        }
+        __syncthreads();
+        const int cols = nh * (HD / 4), groups = cols < PA_WARPS * 32 ? PA_WARPS * 32 / cols : 1;
+        const int per_group = (nc + groups - 1) / groups;
+        float4* sg = reinterpret_cast<float4*>(xo) + (nh * nc + nh + 3) / 4;   // [groups - 1][cols]
+        auto column = [&](int e, int ca, int cb) {
+          const int h = e / (HD / 4), d4 = e % (HD / 4);
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int c = ca; c < cb; ++c) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(row_of(c, h)) + d4);
+            const float wt = sw[h * nc + c];
+            O.x = __fmaf_rn(wt, v.x, O.x); O.y = __fmaf_rn(wt, v.y, O.y);
+            O.z = __fmaf_rn(wt, v.z, O.z); O.w = __fmaf_rn(wt, v.w, O.w);
+          }
+          return O;
+        };
+        auto write = [&](int e, const float4& O) {
+          const int h = e / (HD / 4), d4 = e % (HD / 4);
+          const float L = sl[h], r[4] = {O.x, O.y, O.z, O.w};
+          const long long at = seq * P.o_tok + (h0 + h) * P.o_head + 4 * d4;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) pg_store(P.out, P.type, at + x, L == 0.f ? 0.f : __fdiv_rn(r[x], L) * vscale);
+        };
+        if (groups == 1) {
+          for (int e = tid; e < cols; e += PA_WARPS * 32) write(e, column(e, 0, nc));
+        } else {
+          const int e = tid % cols, gi = tid / cols;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (gi < groups) O = column(e, min(nc, gi * per_group), min(nc, (gi + 1) * per_group));
+          if (gi > 0 && gi < groups) sg[(gi - 1) * cols + e] = O;
+          __syncthreads();
+          if (gi == 0) {
+            for (int x = 0; x + 1 < groups; ++x) {
+              const float4 v = sg[x * cols + e];
+              O.x += v.x; O.y += v.y; O.z += v.z; O.w += v.w;
+            }
+            write(e, O);
+          }
         }
         if (tid == 0) W.ticket[c0] = 0;
       }
