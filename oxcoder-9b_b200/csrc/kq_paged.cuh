@@ -208,8 +208,11 @@ template <int CT, int HD, int NT, bool PREC>
 struct PaShape {
   static constexpr bool BF = CT == PG_BF16;
   static constexpr int ES = CT == PG_E4M3 ? 1 : 2;
+  static constexpr int HEADS = 8 * NT;
   static constexpr int ROW = HD * ES, LD = ROW + 16;           // odd multiples of 16 bytes: conflict-free ldmatrix rows
-  static constexpr int STAGE = 2 * PA_SUB * LD;                // K and V rows of one step of a warp
+  static constexpr int KV = 2 * PA_SUB * LD;                   // K and V rows of one step of a warp
+  static constexpr int QX = HEADS * (HD + 8) * 4;              // a segment's query rows, or a warp's (o, m, l) rows
+  static constexpr int STAGE = KV > QX ? KV : QX;              // a ring slot holds any of the three
   static constexpr int FIT = 104 * 1024 / (PA_WARPS * STAGE);
   static constexpr int STAGES = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;   // two CTAs per SM where three stages leave the room
   static constexpr int KS = HD / 16;
@@ -217,12 +220,10 @@ struct PaShape {
   static constexpr int NP = PREC ? (BF ? 3 : 2) : 2;           // terms of a softmax weight
   static constexpr bool QREG = KS * NQ * NT * 2 <= 64;         // query fragments in registers, else in shared memory
   static constexpr int QBYTES = QREG ? 0 : KS * NQ * NT * 256;
-  static constexpr int HEADS = 8 * NT;
   static constexpr int MLD = HD + 4;                           // row of the warps' exchange: o, m, l
-  static constexpr int RING = PA_WARPS * STAGES * STAGE;
-  static constexpr int XCHG = PA_WARPS * HEADS * MLD * 4;
-  static constexpr int SMEM = (RING > XCHG ? RING : XCHG) + QBYTES;
+  static constexpr int SMEM = PA_WARPS * STAGES * STAGE + QBYTES;
 };
+constexpr int PA_COST = 1;                     // what a (sequence, head) costs beside its tiles, in tiles
 constexpr int PA_PLD = 256 + 4;                // floats of a scratch row (the widest head_dim)
 
 struct AttendScratch {
@@ -230,11 +231,21 @@ struct AttendScratch {
   int* ticket;      // [PA_MAX_CTAS], zero between launches
 };
 
-// The tiles of all (sequence, virtual head, 64-key tile) triples, in this order, are cut into equal
-// runs, one per CTA, wherever sequences end: CTAs finish together whatever the lengths are. A CTA
-// walks its run segment by segment (one sequence and head at a time). A segment that is a whole
-// (sequence, head) is written out; otherwise its (o, m, l) goes to the scratch and the last CTA of
-// the chain to arrive joins the chain's partials in CTA order, so the sums' order is fixed.
+// A cursor over a CTA's run: the units of (sequence, virtual head) are PA_COST empty ones and its tiles.
+struct PaCursor {
+  int seq, head, at, tiles, t0, t1;   // at: unit in the segment; [t0, t1): the run's tiles of this segment
+  long long seg, left;                // first unit of the segment, units left of the run
+  KeyRange R;
+};
+
+// The work is cut into equal runs of units, one per CTA, in the order sequence, head, 64-key tile,
+// wherever sequences end: CTAs finish together whatever the lengths are (cutting by tiles alone left the
+// CTAs with many short sequences 4 times behind the others). A CTA walks its run segment by segment
+// (one sequence and head at a time). Each warp owns a ring of slots and fills it STAGES - 1 steps
+// ahead, across segment borders: a segment's query rows first, then its steps of 16 keys, so nothing
+// but the last slots of a run is waited for in full. A segment that is a whole (sequence, head) is
+// written out; otherwise its (o, m, l) goes to the scratch and the last CTA of the chain to arrive
+// joins the chain's partials in CTA order, so the sums' order is fixed.
 template <int CT, int HD, int NT, bool PREC>
 __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
   using S = PaShape<CT, HD, NT, PREC>;
@@ -242,7 +253,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
   constexpr int KS = S::KS, NQ = S::NQ, NP = S::NP;
   constexpr float PSCALE = BF ? 1.f : 16384.f;   // fp16 weights use 2^14 .. 2^-24: 38 bits below the largest
   extern __shared__ __align__(128) uint8_t pa_smem[];
-  __shared__ long long s_start, s_total;
+  __shared__ __align__(16) float4 s_sum[PA_WARPS * 32];
+  __shared__ float s_M[S::HEADS], s_L[S::HEADS];
+  __shared__ long long s_start;
   __shared__ long long s_scan[PA_WARPS];
   __shared__ int s_seq, s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, t4 = lane & 3;
@@ -252,13 +265,17 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
     R = pg_keys(P, i, false);
     return R.last > R.first ? (R.last - (R.first & ~(PA_SUB - 1)) + PA_TILE - 1) / PA_TILE : 0;
   };
-  // ---- where this CTA's run begins: a scan of the sequences' tiles, consecutive ones per thread
+  auto units_of = [&](int i) {
+    KeyRange R;
+    const int t = tiles_of(i, R);
+    return t ? t + PA_COST : 0;
+  };
+  // ---- where this CTA's run begins: a scan of the sequences' units, consecutive ones per thread
   const int per = (P.n + PA_WARPS * 32 - 1) / (PA_WARPS * 32), i0 = min(P.n, tid * per), i1 = min(P.n, i0 + per);
   long long mine = 0;
   for (int i = i0; i < i1; ++i) {
     if (blockIdx.x == 0) pg_keys(P, i, true);
-    KeyRange R;
-    mine += tiles_of(i, R);
+    mine += units_of(i);
   }
   long long incl = mine;
 #pragma unroll
@@ -280,8 +297,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
   if (begin < end && before * H <= begin && begin < (before + mine) * H) {
     long long b = before;
     for (int i = i0; i < i1; ++i) {
-      KeyRange R;
-      const int u = tiles_of(i, R);
+      const int u = units_of(i);
       if (begin < (b + u) * H) {
         s_seq = i;
         s_start = b * H;
@@ -290,85 +306,127 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
       b += u;
     }
   }
-  if (tid == 0) s_total = total;
   // rows without a key: zeros
   for (int i = blockIdx.x; i < P.n; i += gridDim.x) {
-    KeyRange R;
-    if (tiles_of(i, R)) continue;
+    if (units_of(i)) continue;
     for (int e = tid; e < P.n_heads * HD; e += PA_WARPS * 32) pg_store(P.out, P.type, i * P.o_tok + (e / HD) * P.o_head + e % HD, 0.f);
   }
   __syncthreads();
   if (begin >= end) return;
 
+  // the run's tiles of the segment under the cursor; none if the run ends before its first
+  auto settle = [&](PaCursor& c) {
+    c.t0 = max(0, c.at - PA_COST);
+    c.t1 = (int)min((long long)(c.tiles + PA_COST), c.at + c.left) - PA_COST;
+    if (c.t1 <= c.t0) c.left = 0;
+  };
+  auto next_segment = [&](PaCursor& c) {
+    c.left -= c.t1 + PA_COST - c.at;
+    c.at = 0;
+    c.seg += c.tiles + PA_COST;
+    if (c.left > 0 && ++c.head == H) {
+      c.head = 0;
+      do c.tiles = tiles_of(++c.seq, c.R);
+      while (c.tiles == 0);
+    }
+    settle(c);
+  };
+  PaCursor cur;
+  cur.seq = s_seq;
+  cur.tiles = tiles_of(cur.seq, cur.R);
+  cur.head = (int)((begin - s_start) / (cur.tiles + PA_COST));
+  cur.seg = s_start + (long long)cur.head * (cur.tiles + PA_COST);
+  cur.at = (int)(begin - cur.seg);
+  cur.left = end - begin;
+  settle(cur);
+
+  // ---- the ring's loader
   const uint32_t ring = smem_u32(pa_smem) + warp * S::STAGES * S::STAGE;
-  uint2* qs = reinterpret_cast<uint2*>(pa_smem + (S::SMEM - S::QBYTES));
-  float* xo = reinterpret_cast<float*>(pa_smem);
-  // this lane's part of a step's rows: 16-byte chunks lane, lane + 32, .. of the 16 rows
-  constexpr int CH = S::ROW / 16, NCP = S::ROW / 32;
-  const int lr = lane / CH, lc = lane % CH;            // CH <= 32: row and chunk of the first one
+  constexpr int CH = S::ROW / 16, NCP = S::ROW / 32;   // 16-byte chunks of a row; a lane's chunks of 16 rows
   constexpr int RSTEP = 32 / CH;                       // rows between a lane's chunks
+  const int lr = lane / CH, lc = lane % CH;
+  const int q_es = P.type == PG_F32 ? 4 : 2, q_ld = HD * q_es + 32;
+  PaCursor ld = cur;
+  int ld_tile = ld.t0 - 1;                             // t0 - 1: the query rows
+  uint32_t pages_ok = 0;                               // one bit per slot: its page exists
+  int slot = 0, fill = 0;
+  auto load = [&]() {
+    const uint32_t dst = ring + fill * S::STAGE;
+    if (ld.left > 0) {
+      const int kv = ld.head / HT;
+      if (ld_tile < ld.t0) {
+        const int h0 = kv * G + (ld.head % HT) * S::HEADS, nh = min(S::HEADS, (kv + 1) * G - h0), qc = HD * q_es / 16;
+        const char* q = reinterpret_cast<const char*>(P.q) + (ld.seq * P.q_tok + h0 * P.q_head) * q_es;
+        for (int e = lane; e < nh * qc; e += 32) {
+          const int h = e / qc, c = e % qc;
+          pa_cp16(dst + h * q_ld + c * 16, q + h * P.q_head * q_es + c * 16, 16u);
+        }
+      } else {
+        const int key = (ld.R.first & ~(PA_SUB - 1)) + ld_tile * PA_TILE + warp * PA_SUB;
+        if (key < ld.R.last) {
+          const int page = __ldg(P.T.table + ld.R.row * P.T.ld + (key >> P.T.page_shift));
+          const bool ok = page >= 0 && page < P.T.n_pages;
+          pages_ok = (pages_ok & ~(1u << fill)) | ((uint32_t)ok << fill);
+          if (!ok && lane == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
+          const long long row = (key & ((1 << P.T.page_shift) - 1)) + lr;
+          const char* ks = reinterpret_cast<const char*>(P.kc) + (ok ? (page * P.kp + kv * P.kh + row * P.kr) * S::ES + lc * 16 : 0);
+          const char* vs = reinterpret_cast<const char*>(P.vc) + (ok ? (page * P.vp + kv * P.vh + row * P.vr) * S::ES + lc * 16 : 0);
+          const uint32_t d = dst + lr * S::LD + lc * 16;
+#pragma unroll
+          for (int c = 0; c < NCP; ++c) {
+            const int t = key + lr + c * RSTEP;
+            const bool in = ok && t >= ld.R.first && t < ld.R.last;   // rows outside are not read: they may hold anything
+            pa_cp16(d + c * RSTEP * S::LD, in ? ks + c * RSTEP * P.kr * S::ES : (const char*)P.kc, in ? 16u : 0u);
+            pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, in ? vs + c * RSTEP * P.vr * S::ES : (const char*)P.vc, in ? 16u : 0u);
+          }
+        }
+      }
+      if (++ld_tile == ld.t1) {
+        next_segment(ld);
+        ld_tile = ld.t0 - 1;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    fill = fill + 1 == S::STAGES ? 0 : fill + 1;
+  };
+#pragma unroll 1
+  for (int s = 0; s < S::STAGES - 1; ++s) load();
+  // waits for the next slot, keeps the ring filled, and returns the slot
+  auto step = [&]() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+    __syncwarp();   // every lane's copies are here, and every lane has left the slot that load() fills
+    const int now = slot;
+    slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+    load();
+    return now;
+  };
+
+  uint2* qs = reinterpret_cast<uint2*>(pa_smem + (S::SMEM - S::QBYTES));
   const int mi = lane >> 3, ml = lane & 7;
   const uint32_t k_off = (uint32_t)(((mi & 1) * 8 + ml) * S::LD + (mi >> 1) * 16);
   const uint32_t v_off = (uint32_t)(E8 ? ((mi & 1) * 8 + ml) * S::LD + (mi >> 1) * 16 : ((mi >> 1) * 8 + ml) * S::LD + (mi & 1) * 16) +
                          PA_SUB * S::LD;
-
-  int seq = s_seq;
-  KeyRange R;
-  int tiles = tiles_of(seq, R);
-  long long seg0 = s_start, left = end - begin;        // first tile of (seq, head 0)
-  long long at = begin - seg0;
-  int head = (int)(at / tiles), tile = (int)(at % tiles);
-  while (left > 0) {
-    // ---- one segment: tiles [tile, tile_end) of (seq, head)
-    const int tile_end = (int)min((long long)tiles, tile + left);
-    const int kv = head / HT, h0 = kv * G + (head % HT) * S::HEADS, nh = min(S::HEADS, (kv + 1) * G - h0);
-    const int base = R.first & ~(PA_SUB - 1);
-    const int k_begin = base + tile * PA_TILE + warp * PA_SUB, k_end = min(R.last, base + tile_end * PA_TILE);
-    const int* pt = P.T.table + R.row * P.T.ld;
-    const char* kg = reinterpret_cast<const char*>(P.kc) + kv * P.kh * S::ES;
-    const char* vg = reinterpret_cast<const char*>(P.vc) + kv * P.vh * S::ES;
-    uint32_t pages_ok = 0;                             // one bit per ring slot: its page exists
-    auto load = [&](int key, int slot) {
-      if (key >= k_end) return;
-      const int page = __ldg(pt + (key >> P.T.page_shift));
-      const bool ok = page >= 0 && page < P.T.n_pages;
-      pages_ok = (pages_ok & ~(1u << slot)) | ((uint32_t)ok << slot);
-      if (!ok && lane == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
-      const long long row = (key & ((1 << P.T.page_shift) - 1)) + lr;
-      const char* ks = kg + (ok ? (page * P.kp + row * P.kr) * S::ES + lc * 16 : 0);
-      const char* vs = vg + (ok ? (page * P.vp + row * P.vr) * S::ES + lc * 16 : 0);
-      const uint32_t d = ring + slot * S::STAGE + lr * S::LD + lc * 16;
-#pragma unroll
-      for (int c = 0; c < NCP; ++c) {
-        const int t = key + lr + c * RSTEP;
-        const bool in = ok && t >= R.first && t < R.last;   // rows outside are not read: they may hold anything
-        pa_cp16(d + c * RSTEP * S::LD, in ? ks + c * RSTEP * P.kr * S::ES : kg, in ? 16u : 0u);
-        pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, in ? vs + c * RSTEP * P.vr * S::ES : vg, in ? 16u : 0u);
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < S::STAGES - 1; ++s) {
-      load(k_begin + s * PA_TILE, s);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+  while (cur.left > 0) {
+    const int kv = cur.head / HT, h0 = kv * G + (cur.head % HT) * S::HEADS, nh = min(S::HEADS, (kv + 1) * G - h0);
     // ---- query fragments (column grp of each 8 heads), scaled to [2^9, 2^10) by a power of two
+    const uint8_t* qrow = pa_smem + warp * S::STAGES * S::STAGE + step() * S::STAGE;
     uint32_t qf[S::QREG ? NQ : 1][S::QREG ? NT : 1][S::QREG ? KS : 1][2];
     float sc[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int hh = nt * 8 + grp;
-      const long long qo = seq * P.q_tok + (h0 + min(hh, nh - 1)) * P.q_head;
+      const void* q = qrow + min(hh, nh - 1) * q_ld;
       float mx = 0.f;
 #pragma unroll
       for (int d = 2 * t4; d < HD; d += 8) {
-        const float2 a = pg_load2(P.q, P.type, qo + d);
+        const float2 a = pg_load2(q, P.type, d);
         mx = fmaxf(mx, fmaxf(fabsf(a.x), fabsf(a.y)));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       int e = 0;
       if (mx > 0.f && mx < INFINITY) e = max(-100, (int)((__float_as_uint(mx) >> 23) & 255u) - 127);
-      const float up = hh < nh ? __uint_as_float((uint32_t)(127 + 9 - e) << 23) : 0.f;
+      const float up = __uint_as_float((uint32_t)(127 + 9 - e) << 23);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if (!S::QREG && (ks & 3) != warp) continue;
@@ -377,7 +435,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
           // the dims of k indices 2 t4, 2 t4 + 1 (+ 8): 8-bit K fragments hold dims 4 t4 .. 4 t4 + 3
           const int d = 16 * ks + (E8 ? 4 * t4 + 2 * half : 2 * t4 + 8 * half);
           uint32_t t[NQ];
-          const float2 a = hh < nh ? pg_load2(P.q, P.type, qo + d) : make_float2(0.f, 0.f);
+          const float2 a = hh < nh ? pg_load2(q, P.type, d) : make_float2(0.f, 0.f);
           pa_split<BF, NQ>(a.x * up, a.y * up, t);
 #pragma unroll
           for (int j = 0; j < NQ; ++j) {
@@ -401,16 +459,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
 #pragma unroll
       for (int d = 0; d < KS; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
     }
-    int slot = 0, fill = S::STAGES - 1;
-    for (int key = k_begin; key < k_end; key += PA_TILE) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
-      __syncwarp();
-      const bool ok = (pages_ok >> slot) & 1u;
-      const uint32_t kb = ring + slot * S::STAGE + k_off, vb = ring + slot * S::STAGE + v_off;
-      load(key + (S::STAGES - 1) * PA_TILE, fill);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      fill = slot;
-      slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+    int key = (cur.R.first & ~(PA_SUB - 1)) + cur.t0 * PA_TILE + warp * PA_SUB, now = 0;
+    for (int tile = cur.t0; tile < cur.t1; ++tile, key += PA_TILE) {
+      const bool ok_now = (pages_ok >> slot) & 1u;
+      now = step();
+      if (key >= cur.R.last) continue;
+      const uint32_t kb = ring + now * S::STAGE + k_off, vb = ring + now * S::STAGE + v_off;
       // ---- scores: the terms of the queries in accumulators of their own, smallest added first
       float s[NQ][NT][4];
 #pragma unroll
@@ -449,8 +503,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
         }
       }
       // ---- online softmax, in powers of two: rows (keys) grp and grp + 8, heads 2 t4 and 2 t4 + 1
-      const bool va = ok && key + grp >= R.first && key + grp < R.last;
-      const bool vb8 = ok && key + grp + 8 >= R.first && key + grp + 8 < R.last;
+      const bool va = ok_now && key + grp >= cur.R.first && key + grp < cur.R.last;
+      const bool vb8 = ok_now && key + grp + 8 >= cur.R.first && key + grp + 8 < cur.R.last;
       uint32_t pf[NP][NT][2];
       float f[NT][2];
 #pragma unroll
@@ -520,11 +574,12 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
           accumulate(d, a);
         }
       }
-      __syncwarp();   // the slot may be filled again
     }
-    // ---- join the warps: (o, m, l) rows through the (drained) ring
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+    // ---- join the warps: (o, m, l) rows through the slots just read
+    __syncwarp();
+    auto xrow = [&](int w, int h) {
+      return reinterpret_cast<float*>(pa_smem + (w * S::STAGES + now) * S::STAGE) + h * S::MLD;
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -533,7 +588,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
         ls += __shfl_xor_sync(0xffffffffu, ls, 4);
         ls += __shfl_xor_sync(0xffffffffu, ls, 8);
         ls += __shfl_xor_sync(0xffffffffu, ls, 16);
-        float* row = xo + (warp * S::HEADS + nt * 8 + 2 * t4 + c) * S::MLD;
+        float* row = xrow(warp, nt * 8 + 2 * t4 + c);
         if (grp == 0) {
           row[HD] = m[nt][c];
           row[HD + 1] = ls;
@@ -546,26 +601,24 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
       }
     }
     __syncthreads();
-    const bool whole = tile == 0 && tile_end == tiles;
-    const long long seg_begin = seg0 + (long long)head * tiles;
-    const int slot_id = 2 * blockIdx.x + (tile == 0 ? 1 : 0);
-    float* part = W.part + (size_t)slot_id * PA_MAX_HEADS * PA_PLD;
+    const bool whole = cur.t0 == 0 && cur.t1 == cur.tiles;
+    float* part = W.part + (size_t)(2 * blockIdx.x + (cur.t0 == 0 ? 1 : 0)) * PA_MAX_HEADS * PA_PLD;
     const float vscale = P.vs ? P.vs[kv] : 1.f;
     for (int e = tid; e < nh * HD; e += PA_WARPS * 32) {
       const int h = e / HD, d = e % HD;
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, xo[(w * S::HEADS + h) * S::MLD + HD]);
+      for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, xrow(w, h)[HD]);
       const float u = M == -INFINITY ? 0.f : M;
       float L = 0.f, O = 0.f;
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) {
-        const float* row = xo + (w * S::HEADS + h) * S::MLD;
+        const float* row = xrow(w, h);
         const float wt = exp2f(row[HD] - u);
         L = __fmaf_rn(wt, row[HD + 1], L);
         O = __fmaf_rn(wt, row[d], O);
       }
-      if (whole) pg_store(P.out, P.type, seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
+      if (whole) pg_store(P.out, P.type, cur.seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
       else {
         __stcg(part + h * PA_PLD + d, O);
         if (d == 0) {
@@ -575,49 +628,46 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
       }
     }
     if (!whole) {
-      const int c0 = (int)(seg_begin / run), c1 = (int)((seg_begin + tiles - 1) / run);
+      const int c0 = (int)((cur.seg + PA_COST) / run), c1 = (int)((cur.seg + PA_COST + cur.tiles - 1) / run);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(&W.ticket[c0], 1) == c1 - c0;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        // weights exp2(m_c - M) of the chain's partials, all requested at once; then float4 columns,
-        // the CTAs' rows split over the thread groups a narrow segment leaves idle
+        // the largest m and the sum L of each head, then float4 columns with weights exp2(m_c - M), the
+        // chain's rows split over the thread groups that a narrow segment leaves idle
         const int nc = c1 - c0 + 1;
-        float* sw = xo;                                  // [nh][nc], then L[nh], then the groups' sums
-        float* sl = sw + nh * nc;
         auto row_of = [&](int c, int h) { return W.part + ((size_t)(2 * (c0 + c) + (c == 0)) * PA_MAX_HEADS + h) * PA_PLD; };
         for (int h = warp; h < nh; h += PA_WARPS) {
           float M = -INFINITY, L = 0.f;
-          for (int c = lane; c < nc; c += 32) {
-            const float v = __ldcg(row_of(c, h) + HD);
-            sw[h * nc + c] = v;
-            M = fmaxf(M, v);
-          }
+          for (int c = lane; c < nc; c += 32) M = fmaxf(M, __ldcg(row_of(c, h) + HD));
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
           const float u = M == -INFINITY ? 0.f : M;
           for (int c = lane; c < nc; c += 32) {
-            const float wt = exp2f(sw[h * nc + c] - u);
-            sw[h * nc + c] = wt;
-            L = __fmaf_rn(wt, __ldcg(row_of(c, h) + HD + 1), L);
+            const float2 ml2 = __ldcg(reinterpret_cast<const float2*>(row_of(c, h) + HD));
+            L = __fmaf_rn(exp2f(ml2.x - u), ml2.y, L);
           }
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, off));
-          if (lane == 0) sl[h] = L;
+          if (lane == 0) {
+            s_M[h] = u;
+            s_L[h] = L;
+          }
         }
         __syncthreads();
         const int cols = nh * (HD / 4), groups = cols < PA_WARPS * 32 ? PA_WARPS * 32 / cols : 1;
         const int per_group = (nc + groups - 1) / groups;
-        float4* sg = reinterpret_cast<float4*>(xo) + (nh * nc + nh + 3) / 4;   // [groups - 1][cols]
         auto column = [&](int e, int ca, int cb) {
           const int h = e / (HD / 4), d4 = e % (HD / 4);
+          const float u = s_M[h];
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
           for (int c = ca; c < cb; ++c) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(row_of(c, h)) + d4);
-            const float wt = sw[h * nc + c];
+            const float* row = row_of(c, h);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(row) + d4);
+            const float wt = exp2f(__ldcg(row + HD) - u);
             O.x = __fmaf_rn(wt, v.x, O.x); O.y = __fmaf_rn(wt, v.y, O.y);
             O.z = __fmaf_rn(wt, v.z, O.z); O.w = __fmaf_rn(wt, v.w, O.w);
           }
@@ -625,8 +675,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
         };
         auto write = [&](int e, const float4& O) {
           const int h = e / (HD / 4), d4 = e % (HD / 4);
-          const float L = sl[h], r[4] = {O.x, O.y, O.z, O.w};
-          const long long at = seq * P.o_tok + (h0 + h) * P.o_head + 4 * d4;
+          const float L = s_L[h], r[4] = {O.x, O.y, O.z, O.w};
+          const long long at = cur.seq * P.o_tok + (h0 + h) * P.o_head + 4 * d4;
 #pragma unroll
           for (int x = 0; x < 4; ++x) pg_store(P.out, P.type, at + x, L == 0.f ? 0.f : __fdiv_rn(r[x], L) * vscale);
         };
@@ -636,11 +686,11 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
           const int e = tid % cols, gi = tid / cols;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
           if (gi < groups) O = column(e, min(nc, gi * per_group), min(nc, (gi + 1) * per_group));
-          if (gi > 0 && gi < groups) sg[(gi - 1) * cols + e] = O;
+          if (gi > 0 && gi < groups) s_sum[(gi - 1) * cols + e] = O;
           __syncthreads();
           if (gi == 0) {
             for (int x = 0; x + 1 < groups; ++x) {
-              const float4 v = sg[x * cols + e];
+              const float4 v = s_sum[x * cols + e];
               O.x += v.x; O.y += v.y; O.z += v.z; O.w += v.w;
             }
             write(e, O);
@@ -649,20 +699,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
         if (tid == 0) W.ticket[c0] = 0;
       }
     }
-    __syncthreads();   // the ring and the exchange are free again
-    // ---- next segment
-    left -= tile_end - tile;
-    tile = tile_end;
-    if (tile == tiles) {
-      tile = 0;
-      if (++head == H && left > 0) {
-        head = 0;
-        seg0 += (long long)H * tiles;
-        do tiles = tiles_of(++seq, R);
-        while (tiles == 0);
-      }
-    }
+    __syncthreads();   // the exchange slots are free again
+    next_segment(cur);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 }  // namespace kq
