@@ -247,7 +247,7 @@ struct PaCursor {
 // written out; otherwise its (o, m, l) goes to the scratch and the last CTA of the chain to arrive
 // joins the chain's partials in CTA order, so the sums' order is fixed.
 template <int CT, int HD, int NT, bool PREC>
-__global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
+__global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
   using S = PaShape<CT, HD, NT, PREC>;
   constexpr bool BF = S::BF, E8 = CT == PG_E4M3;
   constexpr int KS = S::KS, NQ = S::NQ, NP = S::NP;
@@ -350,11 +350,25 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
   int ld_tile = ld.t0 - 1;                             // t0 - 1: the query rows
   uint32_t pages_ok = 0;                               // one bit per slot: its page exists
   int slot = 0, fill = 0;
+  // of the loader's segment: this lane's place in row 0 of its head, the table row; and of the next step
+  // its first key and page id (requested a step ahead, so that no copy waits for the table)
+  const char *kseg = nullptr, *vseg = nullptr;
+  const int* tseg = nullptr;
+  int ld_key = 0, ld_page = -1;
+  auto begin_segment = [&]() {
+    const int kv = ld.head / HT;
+    kseg = reinterpret_cast<const char*>(P.kc) + (kv * P.kh + lr * P.kr) * S::ES + lc * 16;
+    vseg = reinterpret_cast<const char*>(P.vc) + (kv * P.vh + lr * P.vr) * S::ES + lc * 16;
+    tseg = P.T.table + ld.R.row * P.T.ld;
+    ld_key = (ld.R.first & ~(PA_SUB - 1)) + ld.t0 * PA_TILE + warp * PA_SUB;
+    ld_tile = ld.t0 - 1;
+  };
+  if (ld.left > 0) begin_segment();
   auto load = [&]() {
     const uint32_t dst = ring + fill * S::STAGE;
     if (ld.left > 0) {
-      const int kv = ld.head / HT;
       if (ld_tile < ld.t0) {
+        const int kv = ld.head / HT;
         const int h0 = kv * G + (ld.head % HT) * S::HEADS, nh = min(S::HEADS, (kv + 1) * G - h0), qc = HD * q_es / 16;
         const char* q = reinterpret_cast<const char*>(P.q) + (ld.seq * P.q_tok + h0 * P.q_head) * q_es;
         for (int e = lane; e < nh * qc; e += 32) {
@@ -362,29 +376,37 @@ __global__ void __launch_bounds__(PA_WARPS * 32) k_page_attend(const __grid_cons
           pa_cp16(dst + h * q_ld + c * 16, q + h * P.q_head * q_es + c * 16, 16u);
         }
       } else {
-        const int key = (ld.R.first & ~(PA_SUB - 1)) + ld_tile * PA_TILE + warp * PA_SUB;
-        if (key < ld.R.last) {
-          const int page = __ldg(P.T.table + ld.R.row * P.T.ld + (key >> P.T.page_shift));
-          const bool ok = page >= 0 && page < P.T.n_pages;
+        if (ld_key < ld.R.last) {
+          const bool ok = ld_page >= 0 && ld_page < P.T.n_pages;
           pages_ok = (pages_ok & ~(1u << fill)) | ((uint32_t)ok << fill);
           if (!ok && lane == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
-          const long long row = (key & ((1 << P.T.page_shift) - 1)) + lr;
-          const char* ks = reinterpret_cast<const char*>(P.kc) + (ok ? (page * P.kp + kv * P.kh + row * P.kr) * S::ES + lc * 16 : 0);
-          const char* vs = reinterpret_cast<const char*>(P.vc) + (ok ? (page * P.vp + kv * P.vh + row * P.vr) * S::ES + lc * 16 : 0);
+          const int row = ld_key & ((1 << P.T.page_shift) - 1);
+          const char* ks = kseg + (ok ? (ld_page * P.kp + row * P.kr) * S::ES : 0);
+          const char* vs = vseg + (ok ? (ld_page * P.vp + row * P.vr) * S::ES : 0);
           const uint32_t d = dst + lr * S::LD + lc * 16;
+          if (ok && ld_key >= ld.R.first && ld_key + PA_SUB <= ld.R.last) {
 #pragma unroll
-          for (int c = 0; c < NCP; ++c) {
-            const int t = key + lr + c * RSTEP;
-            const bool in = ok && t >= ld.R.first && t < ld.R.last;   // rows outside are not read: they may hold anything
-            pa_cp16(d + c * RSTEP * S::LD, in ? ks + c * RSTEP * P.kr * S::ES : (const char*)P.kc, in ? 16u : 0u);
-            pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, in ? vs + c * RSTEP * P.vr * S::ES : (const char*)P.vc, in ? 16u : 0u);
+            for (int c = 0; c < NCP; ++c) {
+              pa_cp16(d + c * RSTEP * S::LD, ks + c * RSTEP * P.kr * S::ES, 16u);
+              pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, vs + c * RSTEP * P.vr * S::ES, 16u);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < NCP; ++c) {
+              const int t = ld_key + lr + c * RSTEP;
+              const bool in = ok && t >= ld.R.first && t < ld.R.last;   // rows outside are not read: they may hold anything
+              pa_cp16(d + c * RSTEP * S::LD, in ? ks + c * RSTEP * P.kr * S::ES : (const char*)P.kc, in ? 16u : 0u);
+              pa_cp16(d + c * RSTEP * S::LD + PA_SUB * S::LD, in ? vs + c * RSTEP * P.vr * S::ES : (const char*)P.vc, in ? 16u : 0u);
+            }
           }
         }
+        ld_key += PA_TILE;
       }
       if (++ld_tile == ld.t1) {
         next_segment(ld);
-        ld_tile = ld.t0 - 1;
+        if (ld.left > 0) begin_segment();
       }
+      if (ld.left > 0 && ld_key < ld.R.last) ld_page = __ldg(tseg + (ld_key >> P.T.page_shift));
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;
