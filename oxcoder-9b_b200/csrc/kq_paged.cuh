@@ -58,6 +58,8 @@ struct AppendParams {
 
 // Grid (token, head row): one CTA turns one head row; thread j its pairs (j, j + rot / 2) and dims.
 __global__ void __launch_bounds__(128) k_page_append(const __grid_constant__ AppendParams P) {
+  pdl_wait();
+  pdl_trigger();
   const int i = blockIdx.x, r = blockIdx.y, half = P.rot / 2;
   const int pos = P.pos[i];
   if (pos < 0) return;
@@ -223,13 +225,19 @@ struct PaShape {
   static constexpr int MLD = HD + 4;                           // row of the warps' exchange: o, m, l
   static constexpr int SMEM = PA_WARPS * STAGES * STAGE + QBYTES;
 };
-constexpr int PA_COST = 1;                     // what a (sequence, head) costs beside its tiles, in tiles
+constexpr int PA_JOIN = 16;                    // partials of a chain read at once
+constexpr int PA_COST = 3;                     // what a (sequence, head) costs beside its tiles, in tiles
 constexpr int PA_PLD = 256 + 4;                // floats of a scratch row (the widest head_dim)
 
 struct AttendScratch {
   float* part;      // [2 * PA_MAX_CTAS][PA_MAX_HEADS][PA_PLD]: o, m, l of a CTA's first (0) and last (1) segment
   int* ticket;      // [PA_MAX_CTAS], zero between launches
 };
+
+// a / b of non-negative numbers, in 32 bits where both fit (the common case; a 64-bit division is slow).
+__device__ __forceinline__ long long pa_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 // A cursor over a CTA's run: the units of (sequence, virtual head) are PA_COST empty ones and its tiles.
 struct PaCursor {
@@ -254,13 +262,15 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   constexpr float PSCALE = BF ? 1.f : 16384.f;   // fp16 weights use 2^14 .. 2^-24: 38 bits below the largest
   extern __shared__ __align__(128) uint8_t pa_smem[];
   __shared__ __align__(16) float4 s_sum[PA_WARPS * 32];
-  __shared__ float s_M[S::HEADS], s_L[S::HEADS];
+  __shared__ float2 s_ml[PA_WARPS * 32];
   __shared__ long long s_start;
   __shared__ long long s_scan[PA_WARPS];
   __shared__ int s_seq, s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, t4 = lane & 3;
   const int G = P.n_heads / P.n_kv, HT = (G + S::HEADS - 1) / S::HEADS, H = P.n_kv * HT;
 
+  pdl_wait();      // everything below may read what the kernels before this one wrote
+  pdl_trigger();   // the next kernel may be scheduled as CTAs leave (it waits for this grid's end itself)
   auto tiles_of = [&](int i, KeyRange& R) {
     R = pg_keys(P, i, false);
     return R.last > R.first ? (R.last - (R.first & ~(PA_SUB - 1)) + PA_TILE - 1) / PA_TILE : 0;
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
     total += s_scan[w];
   }
   total *= H;
-  const long long run = (total + gridDim.x - 1) / gridDim.x;
+  const long long run = pa_div(total + gridDim.x - 1, gridDim.x);
   const long long begin = min(total, blockIdx.x * run), end = min(total, begin + run);
   if (begin < end && before * H <= begin && begin < (before + mine) * H) {
     long long b = before;
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   PaCursor cur;
   cur.seq = s_seq;
   cur.tiles = tiles_of(cur.seq, cur.R);
-  cur.head = (int)((begin - s_start) / (cur.tiles + PA_COST));
+  cur.head = (int)pa_div(begin - s_start, cur.tiles + PA_COST);
   cur.seg = s_start + (long long)cur.head * (cur.tiles + PA_COST);
   cur.at = (int)(begin - cur.seg);
   cur.left = end - begin;
@@ -650,72 +660,82 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
       }
     }
     if (!whole) {
-      const int c0 = (int)((cur.seg + PA_COST) / run), c1 = (int)((cur.seg + PA_COST + cur.tiles - 1) / run);
+      const int c0 = (int)pa_div(cur.seg + PA_COST, run), c1 = (int)pa_div(cur.seg + PA_COST + cur.tiles - 1, run);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(&W.ticket[c0], 1) == c1 - c0;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        // the largest m and the sum L of each head, then float4 columns with weights exp2(m_c - M), the
-        // chain's rows split over the thread groups that a narrow segment leaves idle
-        const int nc = c1 - c0 + 1;
-        auto row_of = [&](int c, int h) { return W.part + ((size_t)(2 * (c0 + c) + (c == 0)) * PA_MAX_HEADS + h) * PA_PLD; };
-        for (int h = warp; h < nh; h += PA_WARPS) {
-          float M = -INFINITY, L = 0.f;
-          for (int c = lane; c < nc; c += 32) M = fmaxf(M, __ldcg(row_of(c, h) + HD));
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-          const float u = M == -INFINITY ? 0.f : M;
-          for (int c = lane; c < nc; c += 32) {
-            const float2 ml2 = __ldcg(reinterpret_cast<const float2*>(row_of(c, h) + HD));
-            L = __fmaf_rn(exp2f(ml2.x - u), ml2.y, L);
-          }
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, off));
-          if (lane == 0) {
-            s_M[h] = u;
-            s_L[h] = L;
-          }
-        }
-        __syncthreads();
-        const int cols = nh * (HD / 4), groups = cols < PA_WARPS * 32 ? PA_WARPS * 32 / cols : 1;
-        const int per_group = (nc + groups - 1) / groups;
+        // float4 columns of the output, PA_JOIN partials of a column requested at a time (a round trip to
+        // the L2 each, which is what a join costs); the chain's rows split over the thread groups that a
+        // narrow segment leaves idle
+        const int nc = c1 - c0 + 1, cols = nh * (HD / 4);
+        const int groups = cols < PA_WARPS * 32 ? PA_WARPS * 32 / cols : 1, per_group = (nc + groups - 1) / groups;
+        float M, L;
+        float4 O;
         auto column = [&](int e, int ca, int cb) {
-          const int h = e / (HD / 4), d4 = e % (HD / 4);
-          const float u = s_M[h];
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int c = ca; c < cb; ++c) {
-            const float* row = row_of(c, h);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(row) + d4);
-            const float wt = exp2f(__ldcg(row + HD) - u);
-            O.x = __fmaf_rn(wt, v.x, O.x); O.y = __fmaf_rn(wt, v.y, O.y);
-            O.z = __fmaf_rn(wt, v.z, O.z); O.w = __fmaf_rn(wt, v.w, O.w);
+          const float* base = W.part + (size_t)(e / (HD / 4)) * PA_PLD;
+          const int d4 = e % (HD / 4);
+          M = -INFINITY;
+          L = 0.f;
+          O = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = ca; c < cb; c += PA_JOIN) {
+            float4 v[PA_JOIN];
+            float2 s2[PA_JOIN];
+            float mx = M;
+#pragma unroll
+            for (int j = 0; j < PA_JOIN; ++j) {
+              const float* row = base + (size_t)(2 * (c0 + c + j) + (c + j == 0)) * PA_MAX_HEADS * PA_PLD;
+              const bool in = c + j < cb;
+              v[j] = in ? __ldcg(reinterpret_cast<const float4*>(row) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+              s2[j] = in ? __ldcg(reinterpret_cast<const float2*>(row + HD)) : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < PA_JOIN; ++j) mx = fmaxf(mx, s2[j].x);
+            const float u = mx == -INFINITY ? 0.f : mx, f = exp2f(M - u);
+            M = mx;
+            L *= f;
+            O.x *= f; O.y *= f; O.z *= f; O.w *= f;
+#pragma unroll
+            for (int j = 0; j < PA_JOIN; ++j) {
+              const float wt = exp2f(s2[j].x - u);
+              L = __fmaf_rn(wt, s2[j].y, L);
+              O.x = __fmaf_rn(wt, v[j].x, O.x); O.y = __fmaf_rn(wt, v[j].y, O.y);
+              O.z = __fmaf_rn(wt, v[j].z, O.z); O.w = __fmaf_rn(wt, v[j].w, O.w);
+            }
           }
-          return O;
         };
-        auto write = [&](int e, const float4& O) {
-          const int h = e / (HD / 4), d4 = e % (HD / 4);
-          const float L = s_L[h], r[4] = {O.x, O.y, O.z, O.w};
-          const long long at = cur.seq * P.o_tok + (h0 + h) * P.o_head + 4 * d4;
+        auto write = [&](int e) {
+          const float r[4] = {O.x, O.y, O.z, O.w};
+          const long long at = cur.seq * P.o_tok + (h0 + e / (HD / 4)) * P.o_head + 4 * (e % (HD / 4));
 #pragma unroll
           for (int x = 0; x < 4; ++x) pg_store(P.out, P.type, at + x, L == 0.f ? 0.f : __fdiv_rn(r[x], L) * vscale);
         };
         if (groups == 1) {
-          for (int e = tid; e < cols; e += PA_WARPS * 32) write(e, column(e, 0, nc));
+          for (int e = tid; e < cols; e += PA_WARPS * 32) {
+            column(e, 0, nc);
+            write(e);
+          }
         } else {
           const int e = tid % cols, gi = tid / cols;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (gi < groups) O = column(e, min(nc, gi * per_group), min(nc, (gi + 1) * per_group));
-          if (gi > 0 && gi < groups) s_sum[(gi - 1) * cols + e] = O;
+          if (gi < groups) column(e, min(nc, gi * per_group), min(nc, (gi + 1) * per_group));
+          if (gi > 0 && gi < groups) {
+            s_sum[tid] = O;
+            s_ml[tid] = make_float2(M, L);
+          }
           __syncthreads();
           if (gi == 0) {
-            for (int x = 0; x + 1 < groups; ++x) {
+            for (int x = 1; x < groups; ++x) {
               const float4 v = s_sum[x * cols + e];
-              O.x += v.x; O.y += v.y; O.z += v.z; O.w += v.w;
+              const float2 s2 = s_ml[x * cols + e];
+              const float mx = fmaxf(M, s2.x), u = mx == -INFINITY ? 0.f : mx, f = exp2f(M - u), wt = exp2f(s2.x - u);
+              M = mx;
+              L = __fmaf_rn(wt, s2.y, L * f);
+              O.x = __fmaf_rn(wt, v.x, O.x * f); O.y = __fmaf_rn(wt, v.y, O.y * f);
+              O.z = __fmaf_rn(wt, v.z, O.z * f); O.w = __fmaf_rn(wt, v.w, O.w * f);
             }
-            write(e, O);
+            write(e);
           }
         }
         if (tid == 0) W.ticket[c0] = 0;

@@ -51,6 +51,8 @@ __global__ void __launch_bounds__(RL_THREADS) k_logit_rules(const __grid_constan
   __shared__ float s_v[RL_THREADS / 32];
   __shared__ int s_i[RL_THREADS / 32];
   const int i = blockIdx.x, tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
   const T* in = reinterpret_cast<const T*>(P.in) + i * P.in_ld;
   T* out = reinterpret_cast<T*>(P.out) + i * P.out_ld;
   const int nh = P.hist ? min(max(P.hist_len[i], 0), P.max_hist) : 0;

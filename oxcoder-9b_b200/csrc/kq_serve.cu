@@ -54,6 +54,23 @@ static AttendKernel attend_kernel(int type, int hd, bool wide, bool prec) {
                                                                              : attend_of<PG_E4M3>(hd, wide, prec);
 }
 
+// Launch with programmatic stream serialisation: the kernel's CTAs may be scheduled while the previous
+// kernel's last ones run; every kernel here begins with the dependency wait, so nothing else changes.
+template <typename... A>
+static cudaError_t launch(void (*fn)(A...), dim3 grid, int threads, size_t smem, void* stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 static int type_size(int type) { return type == KQ_F32 ? 4 : type == KQ_E4M3 ? 1 : 2; }
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 // Strides whose rows all start on 16-byte boundaries and do not run backwards.
@@ -152,8 +169,7 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream
   P.pos = a->pos; P.cos_t = a->cos_t; P.sin_t = a->sin_t; P.rope_ld = a->rope_ld;
   P.n_heads = a->n_heads; P.n_kv = c->d.n_kv_heads; P.hd = c->d.head_dim;
   P.src_type = a->src_type; P.cache_type = c->d.type; P.rot = a->rot; P.n_pos = a->n_pos; P.err = c->dev.err;
-  k_page_append<<<dim3((unsigned)a->n, (unsigned)(a->n_heads + 2 * P.n_kv)), 128, 0, (cudaStream_t)stream>>>(P);
-  CU(cudaGetLastError());
+  CU(launch(k_page_append, dim3((unsigned)a->n, (unsigned)(a->n_heads + 2 * P.n_kv)), 128, 0, stream, P));
   return KQ_OK;
 }
 
@@ -189,8 +205,7 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream
   const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
   const int per_sm = k.smem > 110 * 1024 ? 1 : 2;
   const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * per_sm));
-  k.fn<<<grid, PA_WARPS * 32, k.smem, (cudaStream_t)stream>>>(P, c->scratch);
-  CU(cudaGetLastError());
+  CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, P, c->scratch));
   return KQ_OK;
 }
 
@@ -217,11 +232,8 @@ extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   P.bias_id = a->bias_id; P.bias = a->bias; P.bias_ld = a->bias_ld;
   P.mask = a->mask; P.mask_row = a->mask_row; P.mask_ld = a->mask_ld;
   P.n = a->n; P.vocab = a->vocab; P.max_hist = a->max_hist; P.n_bias = a->n_bias; P.n_masks = a->n_masks; P.err = dev.err;
-  cudaStream_t s = (cudaStream_t)stream;
-  if (a->type == KQ_F32) k_logit_rules<float><<<a->n, RL_THREADS, 0, s>>>(P);
-  else if (a->type == KQ_F16) k_logit_rules<__half><<<a->n, RL_THREADS, 0, s>>>(P);
-  else k_logit_rules<__nv_bfloat16><<<a->n, RL_THREADS, 0, s>>>(P);
-  CU(cudaGetLastError());
+  auto fn = a->type == KQ_F32 ? k_logit_rules<float> : a->type == KQ_F16 ? k_logit_rules<__half> : k_logit_rules<__nv_bfloat16>;
+  CU(launch(fn, dim3((unsigned)a->n), RL_THREADS, 0, stream, P));
   return KQ_OK;
 }
 
