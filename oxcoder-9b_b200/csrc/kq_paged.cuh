@@ -52,56 +52,137 @@ struct AppendParams {
   const int* pos;
   const float *cos_t, *sin_t;
   long long rope_ld;
-  int n_heads, n_kv, hd, src_type, cache_type, rot, n_pos;
+  int n_heads, n_kv, hd, rot, n_pos;
   int* err;
 };
 
-// Grid (token, head row): one CTA turns one head row; thread j its pairs (j, j + rot / 2) and dims.
-__global__ void __launch_bounds__(128) k_page_append(const __grid_constant__ AppendParams P) {
+// V consecutive elements of type T (16 bytes of fp32 or 16-bit elements) as fp32.
+template <int T, int V>
+__device__ __forceinline__ void ap_load(const void* p, float (&x)[V]) {
+  if (T == PG_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = T == PG_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
+                                   : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+// V values rounded to type T; p aligned to the V elements.
+template <int T, int V>
+__device__ __forceinline__ void ap_store(void* p, const float (&x)[V]) {
+  if (T == PG_F32) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  } else if (T == PG_E4M3) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+             (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+    if (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[V / 4 - 1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  } else {
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if (T == PG_F16) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    if (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[V / 2 - 2], w[V / 2 - 1]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
+
+// Bound by memory: each source row is read and each stored row written once, in 16-byte loads. Grid
+// (token, slice of its head rows); a thread owns V pairs (j, j + rot / 2) of one head row, V = 16 bytes
+// of the source type, or 2 V dims that do not turn. The row's loads do not wait for the position;
+// the position, the table entry and the angles follow one another.
+constexpr int AP_THREADS = 128;
+template <int ST, int CT>
+__global__ void __launch_bounds__(AP_THREADS) k_page_append(const __grid_constant__ AppendParams P) {
+  constexpr int V = ST == PG_F32 ? 4 : 8, ES = ST == PG_F32 ? 4 : 2, CS = CT == PG_E4M3 ? 1 : 2;
   pdl_wait();
   pdl_trigger();
-  const int i = blockIdx.x, r = blockIdx.y, half = P.rot / 2;
+  const int i = blockIdx.x, units = P.hd / (2 * V), e = blockIdx.y * AP_THREADS + threadIdx.x;
+  const int r = e / units, u = e % units;
+  if (r >= P.n_heads + 2 * P.n_kv) return;
   const int pos = P.pos[i];
-  if (pos < 0) return;
-  if (P.rot && pos >= P.n_pos) {
-    if (threadIdx.x == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_POS);
-    return;
-  }
   const bool is_q = r < P.n_heads, is_v = r >= P.n_heads + P.n_kv;
   const int h = is_q ? r : is_v ? r - P.n_heads - P.n_kv : r - P.n_heads;
-  const void* src = is_q ? P.q : is_v ? P.v : P.k;
-  const long long so = is_q ? i * P.q_tok + h * P.q_head : is_v ? i * P.v_tok + h * P.v_head : i * P.k_tok + h * P.k_head;
-  void* dst = P.q_out;
-  long long d0 = i * P.o_tok + h * P.o_head;
-  int type = P.src_type;
+  const int half = is_v ? 0 : P.rot / 2;
+  const bool turn = u < half / V;
+  const int j = turn ? u * V : 2 * V * u, j2 = turn ? j + half : j + V;   // the thread's two runs of V dims
+  const char* src = reinterpret_cast<const char*>(is_q ? P.q : is_v ? P.v : P.k) +
+                    (is_q ? i * P.q_tok + h * P.q_head : is_v ? i * P.v_tok + h * P.v_head : i * P.k_tok + h * P.k_head) * ES;
+  float a[V], b[V];
+  ap_load<ST, V>(src + j * ES, a);
+  ap_load<ST, V>(src + j2 * ES, b);
+  if (pos < 0) return;
+  if (P.rot && pos >= P.n_pos) {
+    atomicOr(P.err, KQ_DEV_ERR_BAD_POS);
+    return;
+  }
+  long long page = 0;
   float scale = 1.f;
   if (!is_q) {
     const int s = P.T.seq ? P.T.seq[i] : i, pi = pos >> P.T.page_shift;
     if (s < 0 || s >= P.T.n_seq || pi >= P.T.max_pages) {
-      if (threadIdx.x == 0) atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW : KQ_DEV_ERR_BAD_POS);
+      atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW : KQ_DEV_ERR_BAD_POS);
       return;
     }
-    const int page = P.T.table[s * P.T.ld + pi];
+    page = P.T.table[s * P.T.ld + pi];
     if (page < 0 || page >= P.T.n_pages) {
-      if (threadIdx.x == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
+      atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
       return;
     }
-    const int row = pos & ((1 << P.T.page_shift) - 1);
-    dst = is_v ? P.vc : P.kc;
-    d0 = is_v ? page * P.vp + h * P.vh + row * P.vr : page * P.kp + h * P.kh + row * P.kr;
-    type = P.cache_type;
     const float* sc = is_v ? P.vs : P.ks;
-    if (sc) scale = sc[h];
+    if (CT == PG_E4M3 && sc) scale = sc[h];
   }
-  const int rot = is_v ? 0 : half;
-  for (int j = threadIdx.x; j < rot; j += blockDim.x) {
-    const float a = pg_load(src, P.src_type, so + j), b = pg_load(src, P.src_type, so + j + half);
-    const float c = P.cos_t[pos * P.rope_ld + j], s = P.sin_t[pos * P.rope_ld + j];
-    pg_store(dst, type, d0 + j, __fdiv_rn(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), scale));
-    pg_store(dst, type, d0 + j + half, __fdiv_rn(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)), scale));
+  if (turn) {
+    float c[V], s[V];
+#pragma unroll
+    for (int x = 0; x < V; x += 4) {
+      const float4 cc = *reinterpret_cast<const float4*>(P.cos_t + pos * P.rope_ld + j + x);
+      const float4 ss = *reinterpret_cast<const float4*>(P.sin_t + pos * P.rope_ld + j + x);
+      c[x] = cc.x; c[x + 1] = cc.y; c[x + 2] = cc.z; c[x + 3] = cc.w;
+      s[x] = ss.x; s[x + 1] = ss.y; s[x + 2] = ss.z; s[x + 3] = ss.w;
+    }
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      const float p = a[x], q = b[x];
+      a[x] = __fsub_rn(__fmul_rn(p, c[x]), __fmul_rn(q, s[x]));
+      b[x] = __fadd_rn(__fmul_rn(q, c[x]), __fmul_rn(p, s[x]));
+    }
   }
-  for (int j = 2 * rot + threadIdx.x; j < P.hd; j += blockDim.x)
-    pg_store(dst, type, d0 + j, __fdiv_rn(pg_load(src, P.src_type, so + j), scale));
+  if (is_q) {
+    char* dst = reinterpret_cast<char*>(P.q_out) + (i * P.o_tok + h * P.o_head) * ES;
+    ap_store<ST, V>(dst + j * ES, a);
+    ap_store<ST, V>(dst + j2 * ES, b);
+    return;
+  }
+  if (CT == PG_E4M3) {
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      a[x] = __fdiv_rn(a[x], scale);
+      b[x] = __fdiv_rn(b[x], scale);
+    }
+  }
+  const int row = pos & ((1 << P.T.page_shift) - 1);
+  char* dst = reinterpret_cast<char*>(is_v ? P.vc : P.kc) +
+              (is_v ? page * P.vp + h * P.vh + row * P.vr : page * P.kp + h * P.kh + row * P.kr) * CS;
+  ap_store<CT, V>(dst + j * CS, a);
+  ap_store<CT, V>(dst + j2 * CS, b);
 }
 
 // ------------------------------------------------------------------------------ attention
@@ -416,7 +497,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
         next_segment(ld);
         if (ld.left > 0) begin_segment();
       }
-      if (ld.left > 0 && ld_key < ld.R.last) ld_page = __ldg(tseg + (ld_key >> P.T.page_shift));
+      if (ld.left > 0 && ld_key < ld.R.last) ld_page = tseg[ld_key >> P.T.page_shift];
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;

@@ -54,6 +54,15 @@ static AttendKernel attend_kernel(int type, int hd, bool wide, bool prec) {
                                                                              : attend_of<PG_E4M3>(hd, wide, prec);
 }
 
+typedef void (*AppendFn)(AppendParams);
+template <int ST>
+static AppendFn append_of(int cache) {
+  return cache == KQ_F16 ? k_page_append<ST, PG_F16> : cache == KQ_BF16 ? k_page_append<ST, PG_BF16> : k_page_append<ST, PG_E4M3>;
+}
+static AppendFn append_kernel(int src, int cache) {
+  return src == KQ_F32 ? append_of<PG_F32>(cache) : src == KQ_F16 ? append_of<PG_F16>(cache) : append_of<PG_BF16>(cache);
+}
+
 // Launch with programmatic stream serialisation: the kernel's CTAs may be scheduled while the previous
 // kernel's last ones run; every kernel here begins with the dependency wait, so nothing else changes.
 template <typename... A>
@@ -155,7 +164,7 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream
   REQUIRE(a->rot ? (rows_ok(a->cos_t, a->rope_ld, 0, 4) && rows_ok(a->sin_t, a->rope_ld, 0, 4) && a->rope_ld >= a->rot / 2 && a->n_pos >= 1)
                  : (!a->cos_t && !a->sin_t),
           "kq_page_append: bad rotation table");
-  REQUIRE(a->n_heads + 2 * c->d.n_kv_heads <= 65535, "kq_page_append: too many heads");
+  REQUIRE(a->n_heads <= 65535, "kq_page_append: too many heads");
   if (a->n == 0) return KQ_OK;
   CU(cudaSetDevice(c->device));
   AppendParams P;
@@ -168,8 +177,10 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream
   P.T = table_of(c, a->table, a->seq, a->table_ld, a->n_seq, a->max_pages);
   P.pos = a->pos; P.cos_t = a->cos_t; P.sin_t = a->sin_t; P.rope_ld = a->rope_ld;
   P.n_heads = a->n_heads; P.n_kv = c->d.n_kv_heads; P.hd = c->d.head_dim;
-  P.src_type = a->src_type; P.cache_type = c->d.type; P.rot = a->rot; P.n_pos = a->n_pos; P.err = c->dev.err;
-  CU(launch(k_page_append, dim3((unsigned)a->n, (unsigned)(a->n_heads + 2 * P.n_kv)), 128, 0, stream, P));
+  P.rot = a->rot; P.n_pos = a->n_pos; P.err = c->dev.err;
+  const int units = c->d.head_dim / (a->src_type == KQ_F32 ? 8 : 16), rows = a->n_heads + 2 * P.n_kv;
+  const dim3 grid((unsigned)a->n, (unsigned)((rows * units + AP_THREADS - 1) / AP_THREADS));
+  CU(launch(append_kernel(a->src_type, c->d.type), grid, AP_THREADS, 0, stream, P));
   return KQ_OK;
 }
 
