@@ -9,6 +9,7 @@
 
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <atomic>
 #include <new>
 
 using namespace kq;
@@ -66,17 +67,20 @@ static AppendFn append_kernel(int src, int cache) {
 // Launch with programmatic stream serialisation: the kernel's CTAs may be scheduled while the previous
 // kernel's last ones run; every kernel here begins with the dependency wait, so nothing else changes.
 template <typename... A>
-static cudaError_t launch(void (*fn)(A...), dim3 grid, int threads, size_t smem, void* stream, const A&... args) {
+static cudaError_t launch(void (*fn)(A...), dim3 grid, int threads, size_t smem, void* stream, int cluster, const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
@@ -180,7 +184,7 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream
   P.rot = a->rot; P.n_pos = a->n_pos; P.err = c->dev.err;
   const int units = c->d.head_dim / (a->src_type == KQ_F32 ? 8 : 16), rows = a->n_heads + 2 * P.n_kv;
   const dim3 grid((unsigned)a->n, (unsigned)((rows * units + AP_THREADS - 1) / AP_THREADS));
-  CU(launch(append_kernel(a->src_type, c->d.type), grid, AP_THREADS, 0, stream, P));
+  CU(launch(append_kernel(a->src_type, c->d.type), grid, AP_THREADS, 0, stream, 1, P));
   return KQ_OK;
 }
 
@@ -216,13 +220,30 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream
   const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
   const int per_sm = k.smem > 110 * 1024 ? 1 : 2;
   const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * per_sm));
-  CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, P, c->scratch));
+  CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, 1, P, c->scratch));
+  return KQ_OK;
+}
+
+typedef void (*RulesFn)(RuleParams);
+static RulesFn rules_kernel(int type) {
+  return type == KQ_F32 ? k_logit_rules<float> : type == KQ_F16 ? k_logit_rules<__half> : k_logit_rules<__nv_bfloat16>;
+}
+// Shared memory and cluster sizes above the defaults, allowed once per device (which is current).
+static int rules_setup(int device) {
+  static std::atomic<bool> done[16];
+  if (done[device].load(std::memory_order_acquire)) return KQ_OK;
+  const int smem = (KQ_RULES_MAX_VOCAB / RL_CLUSTER + 16) * 8;
+  for (int type : {KQ_F32, KQ_F16, KQ_BF16}) {
+    CU(cudaFuncSetAttribute(rules_kernel(type), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CU(cudaFuncSetAttribute(rules_kernel(type), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  }
+  done[device].store(true, std::memory_order_release);
   return KQ_OK;
 }
 
 extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   REQUIRE(a, "kq_logit_rules: null argument");
-  REQUIRE(a->n >= 0 && a->vocab >= 1 && a->vocab <= KQ_RULES_MAX_VOCAB, "kq_logit_rules: bad row count or vocabulary size");
+  REQUIRE(a->n >= 0 && a->vocab >= 1 && a->vocab <= KQ_RULES_MAX_VOCAB && a->n <= (1 << 26), "kq_logit_rules: bad row count or vocabulary size");
   REQUIRE(a->type == KQ_F32 || a->type == KQ_F16 || a->type == KQ_BF16, "kq_logit_rules: logits are f32, f16 or bf16");
   const int es = type_size(a->type);
   REQUIRE(a->logits && a->out && aligned(a->logits, es) && aligned(a->out, es) && a->in_ld >= a->vocab && a->out_ld >= a->vocab,
@@ -243,8 +264,16 @@ extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   P.bias_id = a->bias_id; P.bias = a->bias; P.bias_ld = a->bias_ld;
   P.mask = a->mask; P.mask_row = a->mask_row; P.mask_ld = a->mask_ld;
   P.n = a->n; P.vocab = a->vocab; P.max_hist = a->max_hist; P.n_bias = a->n_bias; P.n_masks = a->n_masks; P.err = dev.err;
-  auto fn = a->type == KQ_F32 ? k_logit_rules<float> : a->type == KQ_F16 ? k_logit_rules<__half> : k_logit_rules<__nv_bfloat16>;
-  CU(launch(fn, dim3((unsigned)a->n), RL_THREADS, 0, stream, P));
+  const RulesFn fn = rules_kernel(a->type);
+  // the smallest cluster whose CTAs hold their logits in registers (RL_PRE groups a thread), then larger
+  // ones while the device has CTAs to spare
+  const int vec = 16 / es, reach = a->vocab + vec - 1;
+  int cl = 1;
+  while (cl < RL_CLUSTER && (reach > cl * RL_PRE * RL_THREADS * vec || ((long long)a->n * cl * 2 <= dev.nsm && reach > cl * RL_THREADS * vec))) cl *= 2;
+  P.span = ((reach + cl - 1) / cl + 15) / 16 * 16;
+  const size_t smem = (size_t)P.span * 4 * ((P.hist ? 1 : 0) + (P.n_bias ? 1 : 0));
+  if ((rc = rules_setup(device))) return rc;
+  CU(launch(fn, dim3((unsigned)a->n * (unsigned)cl), RL_THREADS, smem, stream, cl, P));
   return KQ_OK;
 }
 

@@ -27,6 +27,15 @@ def _bind():
     return lib(), check, last_error
 
 
+_rule_call = []
+
+
+def _rules():
+    if not _rule_call:
+        _rule_call.append(_bind()[0].kq_logit_rules)
+    return _rule_call[0]
+
+
 def _type(t):
     c = _types.get(t.dtype)
     if c is None:
@@ -34,16 +43,31 @@ def _type(t):
     return c
 
 
-def _expect(t, what, kind, shape, device):
-    """Pointer of a tensor of this type code (or codes), shape and device whose last dim is dense."""
+def _refuse(t, what, kind, shape, device):
+    """Says why _rows or _vec refused a tensor."""
     if t.get_device() != device:
         raise ValueError("%s is not on device %d" % (what, device))
     if _type(t) != kind:
         raise ValueError("%s has an unsupported or another type: %s" % (what, t.dtype))
     if tuple(t.shape) != shape:
         raise ValueError("%s must have the shape %s, not %s" % (what, shape, tuple(t.shape)))
-    if t.stride(-1) != 1 and shape[-1] > 1:
-        raise ValueError("the last dimension of %s must be dense" % what)
+    raise ValueError("the last dimension of %s must be dense" % what)
+
+
+# These checks are most of what a call costs on the host (a few tenths of a microsecond a tensor, against
+# kernels of a few microseconds), so each looks a property up once.
+def _rows(t, what, kind, shape, device, _codes=_types.get):
+    """(pointer, strides) of a tensor of this type code, shape and device whose last dim is dense."""
+    s = t.stride()
+    if (_codes(t.dtype) != kind and _type(t) != kind) or t.shape != shape or t.get_device() != device or (s[-1] != 1 and shape[-1] > 1):
+        _refuse(t, what, kind, shape, device)
+    return t.data_ptr(), s
+
+
+def _vec(t, what, kind, shape, device, _codes=_types.get):
+    """Pointer of a dense vector of this type code, shape (n,) and device."""
+    if (_codes(t.dtype) != kind and _type(t) != kind) or t.shape != shape or t.get_device() != device or (t.stride()[0] != 1 and shape[0] > 1):
+        _refuse(t, what, kind, shape, device)
     return t.data_ptr()
 
 
@@ -68,12 +92,12 @@ class PagedCache(object):
         self.type = _type(k)
         if self.type not in (F16, BF16, E4M3):
             raise ValueError("pages are float16, bfloat16 or float8_e4m3fn, not %s" % k.dtype)
-        kp = _expect(k, "k", self.type, shape, self.device)
-        vp = _expect(v, "v", self.type, shape, self.device)
-        ks = None if k_scale is None else _expect(k_scale, "k_scale", F32, (self.n_kv,), self.device)
-        vs = None if v_scale is None else _expect(v_scale, "v_scale", F32, (self.n_kv,), self.device)
+        kp, k_st = _rows(k, "k", self.type, shape, self.device)
+        vp, v_st = _rows(v, "v", self.type, shape, self.device)
+        ks = None if k_scale is None else _vec(k_scale, "k_scale", F32, (self.n_kv,), self.device)
+        vs = None if v_scale is None else _vec(v_scale, "v_scale", F32, (self.n_kv,), self.device)
         self.tensors = (k, v, k_scale, v_scale)
-        d = struct.pack("2P6q2P5i4x", kp, vp, *k.stride()[:3], *v.stride()[:3], ks or 0, vs or 0, self.type, self.n_pages,
+        d = struct.pack("2P6q2P5i4x", kp, vp, *k_st[:3], *v_st[:3], ks or 0, vs or 0, self.type, self.n_pages,
                         self.page, self.n_kv, self.hd)
         h = lib.kq_pages_create(d, self.device)
         if not h:
@@ -93,16 +117,17 @@ class PagedCache(object):
             pass
 
     def _table(self, table, seq, n):
-        if len(table.shape) != 2:
+        """Pointers of the table and of the tokens' rows, the table's row stride and shape."""
+        shape = table.shape
+        if len(shape) != 2:
             raise ValueError("the page table must be [sequences, pages]")
-        n_seq, wide = table.shape
-        t = _expect(table, "table", I32, (n_seq, wide), self.device)
-        s = 0
+        n_seq, wide = shape
+        t, s = _rows(table, "table", I32, shape, self.device)
         if seq is not None:
-            s = _expect(seq, "seq", I32, (n,), self.device)
-        elif n > n_seq:
+            return t, _vec(seq, "seq", I32, (n,), self.device), s[0] if n_seq > 1 else wide, n_seq, wide
+        if n > n_seq:
             raise ValueError("more tokens than page-table rows: give seq")
-        return t, s, table.stride(0) if n_seq > 1 else wide, n_seq, wide
+        return t, 0, s[0] if n_seq > 1 else wide, n_seq, wide
 
     def append(self, k, v, table, pos, seq=None, rope=None, q=None, q_out=None, stream=0):
         """K/V rows k, v [n, n_kv_heads, head_dim] (fp32, fp16 or bf16) to positions pos [n] of the sequences whose
@@ -114,32 +139,32 @@ class PagedCache(object):
         n, dev, hd = k.shape[0], self.device, self.hd
         kind = _type(k)
         shape = (n, self.n_kv, hd)
-        kp, vp = _expect(k, "k", kind, shape, dev), _expect(v, "v", kind, shape, dev)
+        kp, (k0, k1, _) = _rows(k, "k", kind, shape, dev)
+        vp, (v0, v1, _) = _rows(v, "v", kind, shape, dev)
         tp, sp, ld, n_seq, wide = self._table(table, seq, n)
-        pp = _expect(pos, "pos", I32, (n,), dev)
+        pp = _vec(pos, "pos", I32, (n,), dev)
         cp = np_ = rot = rl = n_pos = 0
         if rope is not None:
             cos, sin = rope
-            n_pos, half = cos.shape
-            cp, np_ = _expect(cos, "cos", F32, (n_pos, half), dev), _expect(sin, "sin", F32, (n_pos, half), dev)
-            rl, rot = cos.stride(0) if n_pos > 1 else half, 2 * half
-            if n_pos > 1 and sin.stride(0) != rl:
+            shape = cos.shape
+            n_pos, half = shape
+            cp, c_st = _rows(cos, "cos", F32, shape, dev)
+            np_, s_st = _rows(sin, "sin", F32, shape, dev)
+            rl, rot = c_st[0] if n_pos > 1 else half, 2 * half
+            if n_pos > 1 and s_st[0] != rl:
                 raise ValueError("cos and sin must have the same strides")
         qp = op = q0 = q1 = o0 = o1 = heads = 0
         if q is not None:
-            heads = q.shape[1]
             if q_out is None:
                 raise ValueError("queries need q_out")
+            heads = q.shape[1]
             shape = (n, heads, hd)
-            qp, op = _expect(q, "q", kind, shape, dev), _expect(q_out, "q_out", kind, shape, dev)
-            q0, q1, _ = q.stride()
-            o0, o1, _ = q_out.stride()
+            qp, (q0, q1, _) = _rows(q, "q", kind, shape, dev)
+            op, (o0, o1, _) = _rows(q_out, "q_out", kind, shape, dev)
         elif q_out is not None:
             raise ValueError("q_out without q")
         if not n:
             return
-        k0, k1, _ = k.stride()
-        v0, v1, _ = v.stride()
         rc = self._append(self.h, _APPEND.pack(kp, vp, qp, op, k0, k1, v0, v1, q0, q1, o0, o1, tp, sp, pp, cp, np_, ld, rl, n,
                                                heads, kind, n_seq, wide, rot, n_pos), stream)
         if rc:
@@ -151,17 +176,17 @@ class PagedCache(object):
         type (fp32, fp16, bf16), scale: 1 / sqrt(head_dim) by default. A row without positions gives zeros."""
         if not self.h:
             raise ValueError("the cache is closed")
-        n, heads, hd = shape = tuple(q.shape)
+        shape = q.shape
+        n, heads, hd = shape
         dev, kind = self.device, _type(q)
         if hd != self.hd:
             raise ValueError("q has head_dim %d, the cache %d" % (hd, self.hd))
-        qp, op = _expect(q, "q", kind, shape, dev), _expect(out, "out", kind, shape, dev)
+        qp, (q0, q1, _) = _rows(q, "q", kind, shape, dev)
+        op, (o0, o1, _) = _rows(out, "out", kind, shape, dev)
         tp, sp, ld, n_seq, wide = self._table(table, seq, n)
-        lp = _expect(lens, "lens", I32, (n,), dev)
+        lp = _vec(lens, "lens", I32, (n,), dev)
         if not n:
             return out
-        q0, q1, _ = q.stride()
-        o0, o1, _ = out.stride()
         rc = self._attend(self.h, _ATTEND.pack(qp, op, q0, q1, o0, o1, tp, sp, lp, ld, n, heads, kind, n_seq, wide, window,
                                                hd ** -0.5 if scale is None else scale), stream)
         if rc:
@@ -177,36 +202,43 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
     fp32 [n]; bias_ids int32 and bias fp32 [n, entries] (ids outside the vocabulary are padding; the last entry
     of an id stands); mask int32 or uint32 [masks, >= ceil(vocab / 32)], bit id % 32 of word id / 32 set: allowed;
     mask_row [n]: a mask for each row, -1 for none (None: mask i for row i)."""
-    lib, check, _ = _bind()
-    n, vocab = shape = tuple(logits.shape)
+    shape = logits.shape
+    n, vocab = shape
     dev, kind = logits.get_device(), _type(logits)
     if dev < 0:
         raise ValueError("the logits must be on a GPU")
-    ip, op = _expect(logits, "logits", kind, shape, dev), _expect(out, "out", kind, shape, dev)
+    ip, (ild, _) = _rows(logits, "logits", kind, shape, dev)
+    op, (old, _) = _rows(out, "out", kind, shape, dev)
+    if n == 1:
+        ild = old = vocab
     row = (n,)
-    bp = 0 if best is None else _expect(best, "best", I32, row, dev)
+    bp = 0 if best is None else _vec(best, "best", I32, row, dev)
     hp = hl = pl = hld = most = 0
     if hist is not None:
         if hist_len is None:
             raise ValueError("hist needs hist_len")
         most = hist.shape[1]
-        hp, hl = _expect(hist, "hist", I32, (n, most), dev), _expect(hist_len, "hist_len", I32, row, dev)
-        hld = hist.stride(0) if n > 1 else most
+        hp, (hld, _) = _rows(hist, "hist", I32, (n, most), dev)
+        hl = _vec(hist_len, "hist_len", I32, row, dev)
+        if prompt_len is not None:
+            pl = _vec(prompt_len, "prompt_len", I32, row, dev)
+        if n == 1:
+            hld = most
         if not most:
-            hp = hl = 0
+            hp = hl = pl = 0
     elif hist_len is not None or prompt_len is not None:
         raise ValueError("history lengths without a history")
-    if prompt_len is not None:
-        pl = _expect(prompt_len, "prompt_len", I32, row, dev) if hp else 0
-    rp = 0 if repetition is None else _expect(repetition, "repetition", F32, row, dev)
-    fp = 0 if frequency is None else _expect(frequency, "frequency", F32, row, dev)
-    sp = 0 if presence is None else _expect(presence, "presence", F32, row, dev)
+    rp = 0 if repetition is None else _vec(repetition, "repetition", F32, row, dev)
+    fp = 0 if frequency is None else _vec(frequency, "frequency", F32, row, dev)
+    sp = 0 if presence is None else _vec(presence, "presence", F32, row, dev)
     ap = dp = bld = entries = 0
     if bias_ids is not None and bias is not None:
         entries = bias_ids.shape[1]
-        ap, dp = _expect(bias_ids, "bias_ids", I32, (n, entries), dev), _expect(bias, "bias", F32, (n, entries), dev)
-        bld = bias.stride(0) if n > 1 else entries
-        if n > 1 and bias_ids.stride(0) != bld:
+        ap, (bld, _) = _rows(bias_ids, "bias_ids", I32, (n, entries), dev)
+        dp, (vld, _) = _rows(bias, "bias", F32, (n, entries), dev)
+        if n == 1:
+            bld = entries
+        elif bld != vld:
             raise ValueError("bias_ids and bias must have the same strides")
         if not entries:
             ap = dp = 0
@@ -214,22 +246,23 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
         raise ValueError("bias_ids and bias go together")
     mp = mr = mld = masks = 0
     if mask is not None:
-        masks, words = mask.shape
-        mp = _expect(mask, "mask", I32, (masks, words), dev)
-        mld = mask.stride(0) if masks > 1 else words
+        wide = mask.shape
+        masks, words = wide
+        mp, (mld, _) = _rows(mask, "mask", I32, wide, dev)
+        if masks == 1:
+            mld = words
         if words < (vocab + 31) // 32:
             raise ValueError("the masks have too few words")
         if mask_row is not None:
-            mr = _expect(mask_row, "mask_row", I32, row, dev)
+            mr = _vec(mask_row, "mask_row", I32, row, dev)
     elif mask_row is not None:
         raise ValueError("mask_row without masks")
     if not n:
         return out
-    rc = lib.kq_logit_rules(_RULES.pack(ip, op, logits.stride(0) if n > 1 else vocab, out.stride(0) if n > 1 else vocab, bp,
-                                        hp, hl, pl, hld, rp, fp, sp, ap, dp, bld, mp, mr, mld, n, vocab, kind, most, entries,
-                                        masks), dev, stream)
+    rc = _rules()(_RULES.pack(ip, op, ild, old, bp, hp, hl, pl, hld, rp, fp, sp, ap, dp, bld, mp, mr, mld, n, vocab, kind, most,
+                              entries, masks), dev, stream)
     if rc:
-        check(rc)
+        _bind()[1](rc)
     return out
 
 
