@@ -345,6 +345,21 @@ typedef struct {
 } kq_rule_args;
 int kq_logit_rules(const kq_rule_args* a, int device, void* stream);
 
+/* The same operators on tensor objects of a language binding, which would otherwise spend more time on
+ * asking them for their addresses, shapes and strides than the kernels take. kq_tensor_source names the
+ * function that describes an object as a DLPack tensor (PyTorch: dltensor_from_py_object_no_sync of its
+ * DLPack C exchange interface; it must be callable on the calling thread). Objects are passed by address, absent ones
+ * null. Returns KQ_TENSOR_OTHER, with nothing launched, where a description is missing or does not
+ * fit (another device, type or shape): the caller then asks the objects itself and makes the plain call,
+ * whose message says what is wrong. */
+#define KQ_TENSOR_OTHER 1
+int kq_tensor_source(int (*describe)(void* object, void* dl_tensor));
+int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table, void* pos, void* seq, void* cos_t, void* sin_t, void* q,
+                           void* q_out, void* stream);
+int kq_page_attend_tensors(kq_pages* c, void* q, void* table, void* len, void* out, void* seq, int window, float scale, void* stream);
+int kq_logit_rules_tensors(void* logits, void* out, void* best, void* hist, void* hist_len, void* prompt_len, void* repetition,
+                           void* frequency, void* presence, void* bias_id, void* bias, void* mask, void* mask_row, void* stream);
+
 /* Waits for `stream` and reports (and clears) what the operators' kernels flagged on this device. */
 int kq_stream_check(int device, void* stream);
 

@@ -22,7 +22,7 @@ struct RuleParams {
   const int* mask_row;
   long long mask_ld;
   int n, vocab, max_hist, n_bias, n_masks;
-  int span;                  // ids of a row that one CTA of its cluster owns, a multiple of 16
+  int span;                  // ids of a row that one CTA of its cluster owns: whole turns
   int* err;
 };
 
@@ -73,157 +73,263 @@ __device__ __forceinline__ void rl_max(uint32_t a, uint32_t v) {
   asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 
-constexpr int RL_THREADS = 512, RL_PRE = 5, RL_CLUSTER = 16;
+constexpr int RL_THREADS = 512;
+constexpr int RL_CLUSTER = 16;       // CTAs of a row at most
+constexpr int RL_BYTES = 76 * 1024;  // of counts a CTA holds at most if it may: two CTAs per SM
+constexpr int RL_BATCH = 4;          // 16-byte groups of logits a thread requests ahead
+constexpr int RL_TOUCH = 2048;       // touched ids a CTA lists; where there are more it goes through its counts
+constexpr int RL_LIST = 512;         // bias entries of a CTA's ids that it keeps; a longer list is searched where it stands
+constexpr int RL_LOCAL = 16384;      // histories up to here are scanned by every CTA of the row
 
-// Bound by memory: a row is read and written once. A cluster of CTAs owns a row, a CTA `span`
-// consecutive ids of it, with a count and the last bias entry of each id in its shared memory. The
-// history and the bias list are scanned once per row, each CTA a part, the hits sent to the owner's
-// shared memory (integer adds and maxima: their order does not matter). The CTA's logits and mask
-// words are requested into registers before that, RL_PRE 16-byte groups a thread, so the scan runs
-// under their latency. Positions count from the 16-byte boundary at or below the row's start
-// (u = id + shift), so rows of any alignment take 16-byte groups; only a row's ends are handled singly.
-template <typename T>
+// Counts of a CTA's ids in shared memory: 16 bits an id, or 32 where histories may be longer. Beside the
+// count: the id is in the prompt, has a bias.
+template <bool LONG> struct RlCount { using type = uint16_t; static constexpr uint32_t PROMPT = 0x8000u, BIASED = 0x4000u, MOST = 0x3fffu; };
+template <> struct RlCount<true> { using type = uint32_t; static constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, MOST = 0x3fffffffu; };
+
+// Bound by memory: a row is read and written once. A small cluster of CTAs owns a row, its ids dealt out
+// in turns of RL_THREADS 16-byte groups (the frequent ids of a vocabulary lie together: consecutive
+// shares gave one CTA of each row most of the touched ids). First the CTA counts its ids' occurrences in shared memory: a short history is
+// scanned by every CTA of the row (16 KB from the L2 each, no barrier between CTAs), a long one (over
+// RL_LOCAL) by its parts, with the hits sent to the owner's shared memory. The first to count an id
+// lists it, and the listed ids are handled next, a thread each. Then the rest streams through registers,
+// RL_BATCH groups of 16 bytes a thread ahead (the first batch flies during the scan): mask, write, pick.
+// (Touched ids handled within the stream cost every warp their whole latency at almost every step: 128
+// rows with up to 4096 tokens took 124 us; a thread for each token, the first to take an id handling it,
+// 64 to 72.) Counts are integer adds and the last bias entry is a maximum, so nothing depends on the
+// order of arrival.
+// Positions count from the 16-byte boundary at or below the row's start (u = id + shift), so rows of
+// any alignment move in 16-byte groups; only the groups over a row's ends are handled element by element.
+template <typename T, bool LONG>
 __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_constant__ RuleParams P) {
+  using Count = typename RlCount<LONG>::type;
+  using K = RlCount<LONG>;
   constexpr int VEC = 16 / (int)sizeof(T);
-  extern __shared__ __align__(16) uint32_t rl_smem[];
-  __shared__ float s_v[RL_THREADS / 32], s_cv[RL_CLUSTER];
-  __shared__ int s_i[RL_THREADS / 32], s_ci[RL_CLUSTER];
+  extern __shared__ __align__(16) uint8_t rl_smem[];
+  __shared__ float s_v[RL_THREADS / 32], s_cv[RL_CLUSTER], s_bias[RL_LIST];
+  __shared__ int s_i[RL_THREADS / 32], s_ci[RL_CLUSTER], s_entry[RL_LIST], s_id[RL_LIST], s_touched[RL_TOUCH], s_entries, s_n;
   const int tid = threadIdx.x, rank = (int)rl_rank(), ranks = (int)rl_ranks(), i = blockIdx.x / ranks, span = P.span;
-  uint32_t* cnt = rl_smem;
-  uint32_t* last = rl_smem + (P.hist ? span : 0);
+  Count* cnt = reinterpret_cast<Count*>(rl_smem);                                    // [span]
+  const bool counted = P.hist || P.n_bias;
+  if (counted)
+    for (int j = tid; j < span * (int)sizeof(Count) / 16; j += RL_THREADS) reinterpret_cast<uint4*>(cnt)[j] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s_entries = s_n = 0;
   pdl_wait();
   pdl_trigger();
   const T* in = reinterpret_cast<const T*>(P.in) + i * P.in_ld;
   T* out = reinterpret_cast<T*>(P.out) + i * P.out_ld;
   const int shift = (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
-  const bool vec = (int)((reinterpret_cast<uintptr_t>(out) / sizeof(T)) % VEC) == shift;
-  const int u_begin = rank * span, u_end = min(u_begin + span, P.vocab + shift);
+  const bool vec_out = (int)((reinterpret_cast<uintptr_t>(out) / sizeof(T)) % VEC) == shift;
+  // position u is in turn u / STEP, which CTA (turn % ranks) owns as its (turn / ranks)-th; ranks is a power of two
+  constexpr int STEP = RL_THREADS * VEC;
+  const int lg = 31 - __clz(ranks), u_end = P.vocab + shift;
+  auto owner = [&](int u) { return (u / STEP) & (ranks - 1); };
+  auto local = [&](int u) { return ((u / STEP) >> lg) * STEP + (u & (STEP - 1)); };
+  auto place = [&](int turn) { return (turn * ranks + rank) * STEP; };   // where this CTA's turn begins
+  auto whole = [&](int u) { return u >= shift && u + VEC <= u_end; };
+  uint4 x[RL_BATCH];
+  auto request = [&](int turn) {
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k) {
+      const int u = place(turn + k) + tid * VEC;
+      if (whole(u)) x[k] = *reinterpret_cast<const uint4*>(in + (u - shift));
+    }
+  };
+  request(0);
+  const int nh = P.hist ? min(max(P.hist_len[i], 0), P.max_hist) : 0;
+  const int np = P.prompt_len ? P.prompt_len[i] : 0;
   int mrow = P.mask ? (P.mask_row ? P.mask_row[i] : i) : -1;
+  const float rep = P.rep ? P.rep[i] : 1.f, freq = P.freq ? P.freq[i] : 0.f, pres = P.pres ? P.pres[i] : 0.f;
+  const int* hist = P.hist + i * P.hist_ld;
+  const int* bias_id = P.bias_id + i * P.bias_ld;
   const bool none = P.mask && (mrow < -1 || mrow >= P.n_masks);
   if (none) {
     if (tid == 0) atomicOr(P.err, KQ_DEV_ERR_BAD_ROW);
     mrow = -1;
   }
   const uint32_t* mask = mrow >= 0 ? P.mask + mrow * P.mask_ld : nullptr;
-  const int words = (P.vocab + 31) >> 5;
-  // group k of this thread: positions [u, u + VEC); whole: it lies inside the row and both rows are aligned alike
-  auto group = [&](int k) { return u_begin + (k * RL_THREADS + tid) * VEC; };
-  auto whole = [&](int u) { return vec && u >= shift && u + VEC <= u_end; };
-  auto request = [&](int u, uint4& x, uint32_t& m0, uint32_t& m1) {
-    if (whole(u)) x = *reinterpret_cast<const uint4*>(in + (u - shift));
-    m0 = m1 = 0xffffffffu;
-    if (mask && u < u_end) {
-      const int w = max(u - shift, 0) >> 5;
-      m0 = mask[w];
-      m1 = w + 1 < words ? mask[w + 1] : 0u;
+  uint32_t m[RL_BATCH];                                   // the mask word of a group's first id
+  auto request_mask = [&](int turn) {
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k) {
+      const int u = place(turn + k) + tid * VEC;
+      m[k] = mask && u < u_end ? mask[max(u - shift, 0) >> 5] : 0xffffffffu;
     }
   };
-  uint4 x[RL_PRE];
-  uint32_t m0[RL_PRE], m1[RL_PRE];
-#pragma unroll
-  for (int k = 0; k < RL_PRE; ++k) request(group(k), x[k], m0[k], m1[k]);
-
-  const int nh = P.hist ? min(max(P.hist_len[i], 0), P.max_hist) : 0;
-  const int np = P.prompt_len ? P.prompt_len[i] : 0;
-  const bool scan = nh > 0 || P.n_bias > 0;   // the same in all CTAs of the row
-  if (scan) {
-    const int fields = (P.hist ? span : 0) + (P.n_bias ? span : 0);   // span is a multiple of 4
-    for (int j = tid; j < fields / 4; j += RL_THREADS) reinterpret_cast<uint4*>(rl_smem)[j] = make_uint4(0, 0, 0, 0);
-    rl_cluster_sync();                        // every CTA's fields are zero
-    const int* hist = P.hist + i * P.hist_ld;
-    for (int j = rank * RL_THREADS + tid; j < nh; j += ranks * RL_THREADS) {
-      const int id = hist[j];
-      if (id < 0 || id >= P.vocab) continue;
-      const uint32_t u = (uint32_t)(id + shift), r = u / (uint32_t)span, a = rl_at(cnt + (u - r * span), r);
-      if (j < np) rl_or(a, 0x80000000u);
-      else rl_add(a, 1u);
-    }
-    for (int j = rank * RL_THREADS + tid; j < P.n_bias; j += ranks * RL_THREADS) {
-      const int id = P.bias_id[i * P.bias_ld + j];
-      if (id < 0 || id >= P.vocab) continue;
-      const uint32_t u = (uint32_t)(id + shift), r = u / (uint32_t)span;
-      rl_max(rl_at(last + (u - r * span), r), (uint32_t)j + 1u);
-    }
-    rl_cluster_sync();                        // every hit has arrived
-  }
-
-  const float rep = P.rep ? P.rep[i] : 1.f, freq = P.freq ? P.freq[i] : 0.f, pres = P.pres ? P.pres[i] : 0.f;
+  request_mask(0);
   float bv = -INFINITY;
   int bi = 0x7fffffff;
-  auto value = [&](float z, int u, bool allowed) {
-    if (scan) {
-      if (P.hist) z = rl_penalise(z, cnt[u - u_begin], rep, freq, pres);
-      if (P.n_bias) {
-        const uint32_t e = last[u - u_begin];
-        if (e) z = __fadd_rn(z, P.bias[i * P.bias_ld + e - 1]);
-      }
-    }
-    return allowed && !none ? z : -INFINITY;
-  };
-  auto offer = [&](T r, int u) {
-    const float f = rl_get<T>(r);
-    if (f > bv) { bv = f; bi = u - shift; }
-  };
-  auto process = [&](int u, const uint4& v, uint32_t w0, uint32_t w1) {
-    if (u >= u_end) return;
-    const int id0 = u - shift;                // below 0 only in a row's first group
-    if (whole(u)) {
-      const uint32_t ok = (id0 & 31) ? __funnelshift_r(w0, w1, id0 & 31) : w0;
-      union { uint4 q; T t[VEC]; } y;
-      y.q = v;
-      uint32_t any = 0;                       // does a count or a bias touch the group?
-      if (scan) {
-#pragma unroll
-        for (int j = 0; j < VEC; j += 4) {
-          if (P.hist) {
-            const uint4 c = *reinterpret_cast<const uint4*>(cnt + (u - u_begin) + j);
-            any |= c.x | c.y | c.z | c.w;
-          }
-          if (P.n_bias) {
-            const uint4 c = *reinterpret_cast<const uint4*>(last + (u - u_begin) + j);
-            any |= c.x | c.y | c.z | c.w;
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const bool allowed = (ok >> j) & 1u;
-        if (any) y.t[j] = rl_put<T>(value(rl_get<T>(y.t[j]), u + j, allowed));
-        else if (!allowed || none) y.t[j] = rl_put<T>(-INFINITY);
-        offer(y.t[j], u + j);
-      }
-      *reinterpret_cast<uint4*>(out + id0) = y.q;
-      return;
-    }
-    for (int p = max(u, shift); p < min(u + VEC, u_end); ++p) {
-      const int id = p - shift;
-      const T r = rl_put<T>(value(rl_get<T>(in[id]), p, !mask || ((mask[id >> 5] >> (id & 31)) & 1u)));
-      out[id] = r;
-      offer(r, p);
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < RL_PRE; ++k) process(group(k), x[k], m0[k], m1[k]);
-  for (int k = RL_PRE; group(k) < u_end; ++k) {
-    request(group(k), x[0], m0[0], m1[0]);
-    process(group(k), x[0], m0[0], m1[0]);
-  }
-  if (!P.best) return;
-  // ---- the greedy id: warp, CTA, cluster; equal values: the lowest id
-  auto better = [&](float v, int j) {
+  auto better = [&](float v, int j) {                     // equal values: the lowest id
     if (v > bv || (v == bv && j < bi)) { bv = v; bi = j; }
   };
+  auto mine = [&](int id) { return id >= 0 && id < P.vocab && owner(id + shift) == rank; };
+  auto mask_of = [&](int id) { return mask ? mask[id >> 5] : 0xffffffffu; };
+  if (counted) {
+    const bool apart = nh > RL_LOCAL;                     // the same for all CTAs of the row
+    if (apart) rl_cluster_sync();                         // every CTA's counts are zero
+    else __syncthreads();
+    // adds to, or sets bits of, the count of one of this CTA's ids (h < 0: none), and lists it if it was 0; whole warps
+  auto mark = [&](int h, uint32_t v, bool bits) {
+      bool first = false;
+      if (h >= 0) {
+        const int at = local(h + shift), s = LONG ? 0 : 16 * (at & 1);
+        uint32_t* word = reinterpret_cast<uint32_t*>(cnt) + (LONG ? at : at >> 1);
+        const uint32_t old = bits ? atomicOr(word, v << s) : atomicAdd(word, v << s);
+        first = ((old >> s) & (K::PROMPT | K::BIASED | K::MOST)) == 0;
+      }
+      const uint32_t who = __ballot_sync(0xffffffffu, first);
+      int base = 0;
+      if (who && (tid & 31) == 0) base = atomicAdd(&s_n, __popc(who));
+      base = __shfl_sync(0xffffffffu, base, 0) + __popc(who & ((1u << (tid & 31)) - 1u));
+      if (first && base < RL_TOUCH) s_touched[base] = h;
+    };
+    if (apart) {
+      for (int j = rank * RL_THREADS + tid; j < nh; j += ranks * RL_THREADS) {
+        const int h = hist[j];
+        if (h < 0 || h >= P.vocab) continue;
+        const int at = local(h + shift);
+        const uint32_t s = LONG ? 0 : 16 * (at & 1);
+        const uint32_t a = rl_at(reinterpret_cast<uint32_t*>(cnt) + (LONG ? at : at >> 1), (uint32_t)owner(h + shift));
+        if (j < np) rl_or(a, K::PROMPT << s);
+        else rl_add(a, 1u << s);
+      }
+    } else {
+      for (int j0 = 0; j0 < nh; j0 += 4 * RL_THREADS) {
+        int h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = j0 + k * RL_THREADS + tid < nh ? hist[j0 + k * RL_THREADS + tid] : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool old = j0 + k * RL_THREADS + tid < np;
+          if (j0 + k * RL_THREADS < nh) mark(mine(h[k]) ? h[k] : -1, old ? K::PROMPT : 1u, old);
+        }
+      }
+    }
+    for (int j0 = 0; j0 < P.n_bias; j0 += RL_THREADS) {
+      const int j = j0 + tid, h = j < P.n_bias ? bias_id[j] : -1;
+      const bool own_id = mine(h);
+      mark(own_id ? h : -1, K::BIASED, true);
+      if (own_id) {
+        const int e = atomicAdd(&s_entries, 1);
+        if (e < RL_LIST) {
+          s_entry[e] = j;
+          s_id[e] = h;
+          s_bias[e] = P.bias[i * P.bias_ld + j];
+        }
+      }
+    }
+    if (apart) rl_cluster_sync();                         // every hit has arrived
+    else __syncthreads();
+    const int entries = s_entries;
+    auto apply = [&](int h, uint32_t c, float v, uint32_t word) {
+      if (c & ~K::BIASED) v = rl_penalise(v, (c & K::MOST) | ((c & K::PROMPT) ? 0x80000000u : 0u), rep, freq, pres);
+      if (c & K::BIASED) {                                // the last entry of the list with this id
+        int top = -1;
+        float b = 0.f;
+        if (entries <= RL_LIST) {
+          for (int e = 0; e < entries; ++e)
+            if (s_id[e] == h && s_entry[e] > top) {
+              top = s_entry[e];
+              b = s_bias[e];
+            }
+        } else {
+          for (top = P.n_bias - 1; bias_id[top] != h;) --top;
+          b = P.bias[i * P.bias_ld + top];
+        }
+        v = __fadd_rn(v, b);
+      }
+      if (none || !((word >> (h & 31)) & 1u)) v = -INFINITY;
+      const T r = rl_put<T>(v);
+      out[h] = r;
+      const float f = rl_get<T>(r);
+      if (f > -INFINITY) better(f, h);
+    };
+    if (!apart && s_n <= RL_TOUCH) {
+      for (int e = tid; e < s_n; e += RL_THREADS) {
+        const int h = s_touched[e];
+        apply(h, cnt[local(h + shift)], rl_get<T>(in[h]), mask_of(h));
+      }
+    } else {
+      for (int at = tid; at < span; at += RL_THREADS) {
+        const int h = place(at / STEP) + (at & (STEP - 1)) - shift;
+        if (cnt[at]) apply(h, cnt[at], rl_get<T>(in[h]), mask_of(h));
+      }
+    }
+  }
+
+  auto stream = [&](int u, const uint4& v, uint32_t w) {
+    if (u >= u_end) return;
+    const int id0 = u - shift;                            // below 0 only in a row's first group
+    constexpr int CW = VEC * (int)sizeof(Count) / 4;
+    uint32_t c[CW], any = 0;                              // the group's counts
+#pragma unroll
+    for (int j = 0; j < CW; ++j) c[j] = 0;
+    if (counted) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) {
+        const uint2 t = reinterpret_cast<const uint2*>(cnt + local(u))[j / 2];
+        c[j] = t.x;
+        c[j + 1] = t.y;
+        any |= t.x | t.y;
+      }
+    }
+    if (mask) {                                           // bit j: id0 + j is allowed
+      const int e0 = max(id0, 0), s = e0 & 31;
+      uint32_t next = 0;
+      if (s + VEC > 32 && (e0 >> 5) + 1 < (P.vocab + 31) >> 5) next = mask[(e0 >> 5) + 1];
+      w = __funnelshift_r(w, next, s) << (id0 < 0 ? -id0 : 0);
+    }
+    if (none) w = 0;
+    const bool all = whole(u), plain = all && vec_out && !any;
+    union { uint4 q; T t[VEC]; } y;
+    y.q = v;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      if (!all) {
+        if (id0 + j < 0 || u + j >= u_end) continue;
+        y.t[j] = in[id0 + j];
+      }
+      if (!((w >> j) & 1u)) y.t[j] = rl_put<T>(-INFINITY);
+      const float f = rl_get<T>(y.t[j]);
+      const bool clear = LONG ? c[j] == 0 : ((c[j / 2] >> (16 * (j & 1))) & 0xffffu) == 0;
+      if (!plain && clear) out[id0 + j] = y.t[j];         // the touched ids are written already
+      if (clear && f > -INFINITY) better(f, id0 + j);
+    }
+    if (plain) *reinterpret_cast<uint4*>(out + id0) = y.q;
+  };
+#pragma unroll 1
+  for (int turn = 0; place(turn) < u_end; turn += RL_BATCH) {
+    uint4 v[RL_BATCH];
+    uint32_t w[RL_BATCH];
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k) {
+      v[k] = x[k];
+      w[k] = m[k];
+    }
+    request(turn + RL_BATCH);
+    request_mask(turn + RL_BATCH);
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k) stream(place(turn + k) + tid * VEC, v[k], w[k]);
+  }
+  if (!P.best) return;
+  // ---- the greedy id: warp, CTA, cluster
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) better(__shfl_xor_sync(0xffffffffu, bv, off), __shfl_xor_sync(0xffffffffu, bi, off));
   if ((tid & 31) == 0) { s_v[tid >> 5] = bv; s_i[tid >> 5] = bi; }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < RL_THREADS / 32; ++w) better(s_v[w], s_i[w]);
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(rl_at(&s_cv[rank], 0)), "f"(bv) : "memory");
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(rl_at(&s_ci[rank], 0)), "r"(bi) : "memory");
+  if (tid < 32) {
+    bv = tid < RL_THREADS / 32 ? s_v[tid] : -INFINITY;
+    bi = tid < RL_THREADS / 32 ? s_i[tid] : 0x7fffffff;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) better(__shfl_xor_sync(0xffffffffu, bv, off), __shfl_xor_sync(0xffffffffu, bi, off));
+    if (tid == 0) {
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(rl_at(&s_cv[rank], 0)), "f"(bv) : "memory");
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(rl_at(&s_ci[rank], 0)), "r"(bi) : "memory");
+    }
   }
-  rl_cluster_sync();
-  if (rank == 0 && tid == 0) {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (rank != 0) return;                      // nothing reads the other CTAs' shared memory any more
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid == 0) {
     bv = -INFINITY;
     bi = 0x7fffffff;
     for (int r = 0; r < ranks; ++r) better(s_cv[r], s_ci[r]);

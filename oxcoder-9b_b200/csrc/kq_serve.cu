@@ -86,6 +86,8 @@ static cudaError_t launch(void (*fn)(A...), dim3 grid, int threads, size_t smem,
 
 static int type_size(int type) { return type == KQ_F32 ? 4 : type == KQ_E4M3 ? 1 : 2; }
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// A stride of a dimension of one element does not matter.
+static long long stride_of(long long stride, long long size) { return size > 1 ? stride : 0; }
 // Strides whose rows all start on 16-byte boundaries and do not run backwards.
 static bool rows_ok(const void* p, long long a, long long b, int esize) {
   return p && aligned(p, 16) && a >= 0 && b >= 0 && a * esize % 16 == 0 && b * esize % 16 == 0;
@@ -105,8 +107,17 @@ static int pages_check(const kq_page_desc* d) {
   return KQ_OK;
 }
 
-extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) {
+extern "C" kq_pages* kq_pages_create(const kq_page_desc* given, int device) {
   KqhDevice dev;
+  kq_page_desc own{}, *d = nullptr;
+  if (given) {
+    own = *given;
+    own.k_page = stride_of(own.k_page, own.n_pages);
+    own.v_page = stride_of(own.v_page, own.n_pages);
+    own.k_head = stride_of(own.k_head, own.n_kv_heads);
+    own.v_head = stride_of(own.v_head, own.n_kv_heads);
+    d = &own;
+  }
   if (pages_check(d) || kqh_device(device, &dev)) return nullptr;
   kq_pages* c = new (std::nothrow) kq_pages;
   if (!c) {
@@ -153,8 +164,12 @@ static bool table_ok(const kq_pages* c, const int32_t* table, const int32_t* seq
          (long long)max_pages * c->d.page <= 0x7fffffffll;
 }
 
-extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream) {
-  REQUIRE(c && a, "kq_page_append: null argument");
+extern "C" int kq_page_append(kq_pages* c, const kq_append_args* given, void* stream) {
+  REQUIRE(c && given, "kq_page_append: null argument");
+  kq_append_args own = *given, *a = &own;
+  for (long long* x : {&own.k_tok, &own.v_tok, &own.q_tok, &own.o_tok}) *x = stride_of(*x, own.n);
+  for (long long* x : {&own.k_head, &own.v_head}) *x = stride_of(*x, c->d.n_kv_heads);
+  for (long long* x : {&own.q_head, &own.o_head}) *x = stride_of(*x, own.n_heads);
   REQUIRE(a->n >= 0, "kq_page_append: negative token count");
   REQUIRE(a->src_type == KQ_F32 || a->src_type == KQ_F16 || a->src_type == KQ_BF16, "kq_page_append: rows are f32, f16 or bf16");
   const int es = type_size(a->src_type);
@@ -188,8 +203,11 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream
   return KQ_OK;
 }
 
-extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream) {
-  REQUIRE(c && a, "kq_page_attend: null argument");
+extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* stream) {
+  REQUIRE(c && given, "kq_page_attend: null argument");
+  kq_attend_args own = *given, *a = &own;
+  for (long long* x : {&own.q_tok, &own.o_tok}) *x = stride_of(*x, own.n);
+  for (long long* x : {&own.q_head, &own.o_head}) *x = stride_of(*x, own.n_heads);
   REQUIRE(a->n >= 0, "kq_page_attend: negative token count");
   REQUIRE(a->type == KQ_F32 || a->type == KQ_F16 || a->type == KQ_BF16, "kq_page_attend: queries are f32, f16 or bf16");
   const int es = type_size(a->type);
@@ -225,18 +243,20 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream
 }
 
 typedef void (*RulesFn)(RuleParams);
-static RulesFn rules_kernel(int type) {
-  return type == KQ_F32 ? k_logit_rules<float> : type == KQ_F16 ? k_logit_rules<__half> : k_logit_rules<__nv_bfloat16>;
+static RulesFn rules_kernel(int type, bool deep) {
+  if (deep) return type == KQ_F32 ? k_logit_rules<float, true> : type == KQ_F16 ? k_logit_rules<__half, true> : k_logit_rules<__nv_bfloat16, true>;
+  return type == KQ_F32 ? k_logit_rules<float, false> : type == KQ_F16 ? k_logit_rules<__half, false> : k_logit_rules<__nv_bfloat16, false>;
 }
 // Shared memory and cluster sizes above the defaults, allowed once per device (which is current).
 static int rules_setup(int device) {
   static std::atomic<bool> done[16];
   if (done[device].load(std::memory_order_acquire)) return KQ_OK;
-  const int smem = (KQ_RULES_MAX_VOCAB / RL_CLUSTER + 16) * 8;
-  for (int type : {KQ_F32, KQ_F16, KQ_BF16}) {
-    CU(cudaFuncSetAttribute(rules_kernel(type), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    CU(cudaFuncSetAttribute(rules_kernel(type), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  }
+  const int smem = (KQ_RULES_MAX_VOCAB / RL_CLUSTER + 2 * RL_THREADS * 8) * 4;
+  for (int type : {KQ_F32, KQ_F16, KQ_BF16})
+    for (bool deep : {false, true}) {
+      CU(cudaFuncSetAttribute(rules_kernel(type, deep), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      CU(cudaFuncSetAttribute(rules_kernel(type, deep), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    }
   done[device].store(true, std::memory_order_release);
   return KQ_OK;
 }
@@ -264,17 +284,157 @@ extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   P.bias_id = a->bias_id; P.bias = a->bias; P.bias_ld = a->bias_ld;
   P.mask = a->mask; P.mask_row = a->mask_row; P.mask_ld = a->mask_ld;
   P.n = a->n; P.vocab = a->vocab; P.max_hist = a->max_hist; P.n_bias = a->n_bias; P.n_masks = a->n_masks; P.err = dev.err;
-  const RulesFn fn = rules_kernel(a->type);
-  // the smallest cluster whose CTAs hold their logits in registers (RL_PRE groups a thread), then larger
-  // ones while the device has CTAs to spare
-  const int vec = 16 / es, reach = a->vocab + vec - 1;
+  // 32-bit counts only where a history may hold more of one id than 14 bits count. The smallest
+  // cluster whose CTAs hold at most RL_BYTES, then larger ones while the device has CTAs to spare.
+  const bool deep = a->max_hist > (int)RlCount<false>::MOST;
+  const int vec = 16 / es, reach = a->vocab + vec - 1, bytes = !P.hist && !P.n_bias ? 0 : deep ? 4 : 2;
   int cl = 1;
-  while (cl < RL_CLUSTER && (reach > cl * RL_PRE * RL_THREADS * vec || ((long long)a->n * cl * 2 <= dev.nsm && reach > cl * RL_THREADS * vec))) cl *= 2;
-  P.span = ((reach + cl - 1) / cl + 15) / 16 * 16;
-  const size_t smem = (size_t)P.span * 4 * ((P.hist ? 1 : 0) + (P.n_bias ? 1 : 0));
+  while (cl < RL_CLUSTER && ((long long)reach * bytes > (long long)cl * RL_BYTES ||
+                             ((long long)a->n * cl * 2 <= 2 * dev.nsm && reach > cl * RL_THREADS * vec)))
+    cl *= 2;
+  const int turn = RL_THREADS * vec;
+  P.span = (reach + cl * turn - 1) / (cl * turn) * turn;
   if ((rc = rules_setup(device))) return rc;
-  CU(launch(fn, dim3((unsigned)a->n * (unsigned)cl), RL_THREADS, smem, stream, cl, P));
+  CU(launch(rules_kernel(a->type, deep), dim3((unsigned)a->n * (unsigned)cl), RL_THREADS, (size_t)P.span * bytes, stream, cl, P));
   return KQ_OK;
+}
+
+// ------------------------------------------------------------------------------ tensor objects
+// DLPack's DLTensor (its version 1 ABI).
+struct DlTensor {
+  void* data;
+  int32_t device_type, device_id;   // 2: CUDA
+  int32_t ndim;
+  uint8_t code, bits;               // 0 int, 1 uint, 2 float, 4 bfloat, 10 float8_e4m3fn
+  uint16_t lanes;
+  int64_t* shape;
+  int64_t* strides;                 // null: dense
+  uint64_t byte_offset;
+};
+typedef int (*DescribeFn)(void*, void*);
+static std::atomic<DescribeFn> g_describe;
+
+extern "C" int kq_tensor_source(int (*describe)(void*, void*)) {
+  g_describe.store(describe, std::memory_order_release);
+  return KQ_OK;
+}
+
+constexpr int T_I32 = 100;
+struct Tensor {
+  void* p = nullptr;
+  int type = -1, device = -1;
+  long long n[3] = {0, 0, 0}, s[3] = {0, 0, 0};
+};
+// The tensor behind `object`, if it is a CUDA tensor of `nd` dimensions without empty ones, dense in the last.
+static bool tensor_of(void* object, int nd, Tensor& t) {
+  const DescribeFn describe = g_describe.load(std::memory_order_acquire);
+  DlTensor d{};
+  if (!describe || !object || describe(object, &d) != 0 || d.device_type != 2 || d.ndim != nd || d.lanes != 1 || !d.data) return false;
+  t.p = static_cast<char*>(d.data) + d.byte_offset;
+  t.device = d.device_id;
+  t.type = d.code == 2 && d.bits == 32 ? KQ_F32 : d.code == 2 && d.bits == 16 ? KQ_F16 : d.code == 4 && d.bits == 16 ? KQ_BF16
+           : d.code <= 1 && d.bits == 32 ? T_I32 : -1;
+  long long dense = 1;
+  for (int i = nd - 1; i >= 0; --i) {
+    t.n[i] = d.shape[i];
+    t.s[i] = d.strides ? d.strides[i] : dense;
+    dense *= d.shape[i];
+    if (t.n[i] < 1 || t.n[i] > 0x7fffffffll) return false;
+  }
+  return t.s[nd - 1] == 1 || t.n[nd - 1] == 1;
+}
+static bool tensor_as(void* object, const Tensor& like, Tensor& t, int nd) {   // the same type, device and shape
+  return tensor_of(object, nd, t) && t.type == like.type && t.device == like.device && t.n[0] == like.n[0] &&
+         (nd < 2 || t.n[1] == like.n[1]) && (nd < 3 || t.n[2] == like.n[2]);
+}
+static bool vector_as(void* object, int type, int device, long long n, Tensor& t) {
+  return tensor_of(object, 1, t) && t.type == type && t.device == device && t.n[0] == n;
+}
+#define FITS(cond)                     \
+  do {                                 \
+    if (!(cond)) return KQ_TENSOR_OTHER; \
+  } while (0)
+
+extern "C" int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table, void* pos, void* seq, void* cos_t, void* sin_t,
+                                      void* q, void* q_out, void* stream) {
+  FITS(c && !cos_t == !sin_t && !q == !q_out);
+  const int dev = c->device;
+  Tensor tk, tv, tt, tp, ts, tc, tsn, tq, to;
+  FITS(tensor_of(k, 3, tk) && tk.device == dev && tk.n[1] == c->d.n_kv_heads && tk.n[2] == c->d.head_dim && tensor_as(v, tk, tv, 3));
+  const long long n = tk.n[0];
+  FITS(tensor_of(table, 2, tt) && tt.type == T_I32 && tt.device == dev && vector_as(pos, T_I32, dev, n, tp));
+  if (seq) FITS(vector_as(seq, T_I32, dev, n, ts));
+  else FITS(n <= tt.n[0]);
+  if (cos_t)
+    FITS(tensor_of(cos_t, 2, tc) && tc.type == KQ_F32 && tc.device == dev && tensor_as(sin_t, tc, tsn, 2) &&
+         (tc.n[0] == 1 || tc.s[0] == tsn.s[0]));
+  if (q)
+    FITS(tensor_of(q, 3, tq) && tq.type == tk.type && tq.device == dev && tq.n[0] == n && tq.n[2] == tk.n[2] && tensor_as(q_out, tq, to, 3));
+  kq_append_args a{};
+  a.k = tk.p; a.v = tv.p; a.q = tq.p; a.q_out = to.p;
+  a.k_tok = tk.s[0]; a.k_head = tk.s[1]; a.v_tok = tv.s[0]; a.v_head = tv.s[1];
+  a.q_tok = tq.s[0]; a.q_head = tq.s[1]; a.o_tok = to.s[0]; a.o_head = to.s[1];
+  a.table = static_cast<int32_t*>(tt.p); a.seq = static_cast<int32_t*>(ts.p); a.pos = static_cast<int32_t*>(tp.p);
+  a.cos_t = static_cast<float*>(tc.p); a.sin_t = static_cast<float*>(tsn.p);
+  a.table_ld = tt.n[0] > 1 ? tt.s[0] : tt.n[1];
+  a.rope_ld = tc.n[0] > 1 ? tc.s[0] : tc.n[1];
+  a.n = (int)n; a.n_heads = (int)tq.n[1]; a.src_type = tk.type;
+  a.n_seq = (int)tt.n[0]; a.max_pages = (int)tt.n[1];
+  a.rot = (int)(2 * tc.n[1]); a.n_pos = (int)tc.n[0];
+  return kq_page_append(c, &a, stream);
+}
+
+extern "C" int kq_page_attend_tensors(kq_pages* c, void* q, void* table, void* len, void* out, void* seq, int window, float scale,
+                                      void* stream) {
+  FITS(c);
+  const int dev = c->device;
+  Tensor tq, to, tt, tl, ts;
+  FITS(tensor_of(q, 3, tq) && tq.device == dev && tq.n[2] == c->d.head_dim && tensor_as(out, tq, to, 3));
+  const long long n = tq.n[0];
+  FITS(tensor_of(table, 2, tt) && tt.type == T_I32 && tt.device == dev && vector_as(len, T_I32, dev, n, tl));
+  if (seq) FITS(vector_as(seq, T_I32, dev, n, ts));
+  else FITS(n <= tt.n[0]);
+  kq_attend_args a{};
+  a.q = tq.p; a.out = to.p;
+  a.q_tok = tq.s[0]; a.q_head = tq.s[1]; a.o_tok = to.s[0]; a.o_head = to.s[1];
+  a.table = static_cast<int32_t*>(tt.p); a.seq = static_cast<int32_t*>(ts.p); a.len = static_cast<int32_t*>(tl.p);
+  a.table_ld = tt.n[0] > 1 ? tt.s[0] : tt.n[1];
+  a.n = (int)n; a.n_heads = (int)tq.n[1]; a.type = tq.type;
+  a.n_seq = (int)tt.n[0]; a.max_pages = (int)tt.n[1]; a.window = window; a.scale = scale;
+  return kq_page_attend(c, &a, stream);
+}
+
+extern "C" int kq_logit_rules_tensors(void* logits, void* out, void* best, void* hist, void* hist_len, void* prompt_len,
+                                      void* repetition, void* frequency, void* presence, void* bias_id, void* bias, void* mask,
+                                      void* mask_row, void* stream) {
+  FITS(!hist == !hist_len && (hist || !prompt_len) && !bias_id == !bias && (mask || !mask_row));
+  Tensor tl, to, tb, th, thl, tp, tr, tf, ts, ti, tv, tm, tmr;
+  FITS(tensor_of(logits, 2, tl) && tensor_as(out, tl, to, 2));
+  const int dev = tl.device;
+  const long long n = tl.n[0];
+  if (best) FITS(vector_as(best, T_I32, dev, n, tb));
+  if (hist) FITS(tensor_of(hist, 2, th) && th.type == T_I32 && th.device == dev && th.n[0] == n && vector_as(hist_len, T_I32, dev, n, thl));
+  if (prompt_len) FITS(vector_as(prompt_len, T_I32, dev, n, tp));
+  if (repetition) FITS(vector_as(repetition, KQ_F32, dev, n, tr));
+  if (frequency) FITS(vector_as(frequency, KQ_F32, dev, n, tf));
+  if (presence) FITS(vector_as(presence, KQ_F32, dev, n, ts));
+  if (bias)
+    FITS(tensor_of(bias_id, 2, ti) && ti.type == T_I32 && ti.device == dev && ti.n[0] == n && tensor_of(bias, 2, tv) &&
+         tv.type == KQ_F32 && tv.device == dev && tv.n[0] == n && tv.n[1] == ti.n[1] && (n == 1 || tv.s[0] == ti.s[0]));
+  if (mask) FITS(tensor_of(mask, 2, tm) && tm.type == T_I32 && tm.device == dev);
+  if (mask_row) FITS(vector_as(mask_row, T_I32, dev, n, tmr));
+  kq_rule_args a{};
+  auto ld = [](const Tensor& t) { return t.n[0] > 1 ? t.s[0] : t.n[1]; };
+  a.logits = tl.p; a.out = to.p; a.in_ld = ld(tl); a.out_ld = ld(to);
+  a.best = static_cast<int32_t*>(tb.p);
+  a.hist = static_cast<int32_t*>(th.p); a.hist_len = static_cast<int32_t*>(thl.p); a.prompt_len = static_cast<int32_t*>(tp.p);
+  a.hist_ld = ld(th);
+  a.repetition = static_cast<float*>(tr.p); a.frequency = static_cast<float*>(tf.p); a.presence = static_cast<float*>(ts.p);
+  a.bias_id = static_cast<int32_t*>(ti.p); a.bias = static_cast<float*>(tv.p); a.bias_ld = ld(ti);
+  a.mask = static_cast<uint32_t*>(tm.p); a.mask_row = static_cast<int32_t*>(tmr.p); a.mask_ld = ld(tm);
+  a.n = (int)n; a.vocab = (int)tl.n[1]; a.type = tl.type;
+  a.max_hist = (int)th.n[1]; a.n_bias = (int)ti.n[1]; a.n_masks = (int)tm.n[0];
+  return kq_logit_rules(&a, dev, stream);
 }
 
 extern "C" int kq_stream_check(int device, void* stream) {

@@ -105,6 +105,10 @@ SIGNATURES = {
     "kq_page_append": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p]),
     "kq_page_attend": (C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p]),
     "kq_logit_rules": (C.c_int, [C.c_char_p, C.c_int, C.c_void_p]),
+    "kq_tensor_source": (C.c_int, [C.c_void_p]),
+    "kq_page_append_tensors": (C.c_int, [C.c_void_p] * 11),
+    "kq_page_attend_tensors": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_float, C.c_void_p]),
+    "kq_logit_rules_tensors": (C.c_int, [C.c_void_p] * 14),
     "kq_stream_check": (C.c_int, [C.c_int, C.c_void_p]),
     "kq_ngram_create": (C.c_void_p, [C.c_int, C.c_int]),
     "kq_ngram_free": (None, [C.c_void_p]),

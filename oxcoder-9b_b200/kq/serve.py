@@ -22,6 +22,41 @@ _ATTEND = struct.Struct("2P4q3Pq6if4x")
 _RULES = struct.Struct("2P2qP3Pq3P2Pq2Pq6i")
 
 
+class _Direct(object):
+    """The library's calls on tensor objects (kq_*_tensors) for a tensor type that has DLPack's C exchange
+    interface, or None of them: those calls answer OTHER for whatever they cannot take, and the checks
+    below then say why. They keep Python's lock (the interface needs it)."""
+    OTHER = 1
+    type = None
+    _tried = set()
+
+    @classmethod
+    def try_type(cls, t):
+        if t in cls._tried:
+            return
+        cls._tried.add(t)
+        capsule = getattr(t, "__dlpack_c_exchange_api__", None)
+        if cls.type is not None or capsule is None:
+            return
+        from . import LIB_PATH, SIGNATURES
+        get = C.pythonapi.PyCapsule_GetPointer
+        get.restype, get.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+        api = get(capsule, b"dlpack_exchange_api")
+        if C.c_uint32.from_address(api).value != 1:     # the interface's major version
+            return
+        describe = C.c_void_p.from_address(api + 5 * 8).value   # dltensor_from_py_object_no_sync
+        if not describe:
+            return
+        lib = C.PyDLL(LIB_PATH)
+        lib.kq_tensor_source.argtypes = [C.c_void_p]
+        lib.kq_tensor_source(describe)
+        for name in ("kq_page_append_tensors", "kq_page_attend_tensors", "kq_logit_rules_tensors"):
+            f = getattr(lib, name)
+            f.restype, f.argtypes = SIGNATURES[name]
+            setattr(cls, name[3:-8], f)
+        cls.type = t
+
+
 def _bind():
     from . import check, last_error, lib
     return lib(), check, last_error
@@ -83,6 +118,7 @@ class PagedCache(object):
         self.h = None
         self._check = check
         self._free = lib.kq_pages_free
+        _Direct.try_type(type(k))
         if len(k.shape) != 4:
             raise ValueError("K pages must be [n_pages, n_kv_heads, page, head_dim]")
         self.device = k.get_device()
@@ -136,6 +172,16 @@ class PagedCache(object):
         head_dim] into q_out (may be q). pos < 0 skips a token. Slots of one call must be distinct."""
         if not self.h:
             raise ValueError("the cache is closed")
+        T = _Direct.type
+        if type(k) is T and type(v) is T and type(table) is T and type(pos) is T and (rope is None or (type(rope[0]) is T and type(rope[1]) is T)) \
+                and (seq is None or type(seq) is T) and (q is None or (type(q) is T and type(q_out) is T)):
+            rc = _Direct.page_append(self.h, id(k), id(v), id(table), id(pos), None if seq is None else id(seq),
+                                     None if rope is None else id(rope[0]), None if rope is None else id(rope[1]),
+                                     None if q is None else id(q), None if q_out is None else id(q_out), stream)
+            if not rc:
+                return
+            if rc != _Direct.OTHER:
+                self._check(rc)
         n, dev, hd = k.shape[0], self.device, self.hd
         kind = _type(k)
         shape = (n, self.n_kv, hd)
@@ -176,6 +222,14 @@ class PagedCache(object):
         type (fp32, fp16, bf16), scale: 1 / sqrt(head_dim) by default. A row without positions gives zeros."""
         if not self.h:
             raise ValueError("the cache is closed")
+        T = _Direct.type
+        if type(q) is T and type(table) is T and type(lens) is T and type(out) is T and (seq is None or type(seq) is T):
+            rc = _Direct.page_attend(self.h, id(q), id(table), id(lens), id(out), None if seq is None else id(seq), window,
+                                     self.hd ** -0.5 if scale is None else scale, stream)
+            if not rc:
+                return out
+            if rc != _Direct.OTHER:
+                self._check(rc)
         shape = q.shape
         n, heads, hd = shape
         dev, kind = self.device, _type(q)
@@ -202,6 +256,26 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
     fp32 [n]; bias_ids int32 and bias fp32 [n, entries] (ids outside the vocabulary are padding; the last entry
     of an id stands); mask int32 or uint32 [masks, >= ceil(vocab / 32)], bit id % 32 of word id / 32 set: allowed;
     mask_row [n]: a mask for each row, -1 for none (None: mask i for row i)."""
+    T = _Direct.type
+    if type(logits) is not T:
+        _Direct.try_type(type(logits))
+        T = _Direct.type
+    given = (logits, out, best, hist, hist_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, mask_row)
+    if type(logits) is T:
+        ids = []
+        for t in given:
+            if t is None:
+                ids.append(None)
+            elif type(t) is T:
+                ids.append(id(t))
+            else:
+                break
+        else:
+            rc = _Direct.logit_rules(*ids, stream)
+            if not rc:
+                return out
+            if rc != _Direct.OTHER:
+                _bind()[1](rc)
     shape = logits.shape
     n, vocab = shape
     dev, kind = logits.get_device(), _type(logits)

@@ -461,3 +461,35 @@ def test_refusals(env):
     with pytest.raises(ValueError):
         c.attend(q, table, lens, torch.empty_like(q))
     K.check_stream()
+
+
+def test_both_ways_of_passing_tensors_agree(env, monkeypatch):
+    """The short way (DLPack descriptions read by the library) and the checks in Python make the same call."""
+    K, torch = env
+    from kq import serve
+    g = torch.Generator(device="cuda").manual_seed(9)
+    t = dict(dtype=torch.int32, device="cuda")
+    for n, kv, G in ((1, 1, 1), (1, 2, 3), (5, 1, 4), (4, 3, 1)):
+        rows = torch.randn((n, 2 * kv + kv * G + 1, 64), device="cuda", generator=g)
+        kn, vn, q = rows[:, :kv], rows[:, kv:2 * kv], rows[:, 2 * kv:2 * kv + kv * G]
+        big = torch.arange(40, **t).view(5, 8)
+        table, seq = big[:n, 1:5], torch.arange(n, **t).flip(0).contiguous()
+        pos = torch.tensor([3 + 11 * i for i in range(n)], **t)
+        cos, sin = rope_tables(torch, 64, 32)
+        got = []
+        for direct in (True, False):
+            monkeypatch.setattr(serve._Direct, "type", torch.Tensor if direct else None)
+            monkeypatch.setattr(serve._Direct, "_tried", {torch.Tensor})
+            k, v = (torch.zeros((40, kv, 16, 64), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+            c = K.PagedCache(k, v)
+            qo, out = torch.zeros_like(q), torch.zeros_like(q)
+            c.append(kn, vn, table, pos, seq=seq, rope=(cos, sin), q=q, q_out=qo)
+            c.attend(qo, table, pos + 1, out, seq=seq, window=9, scale=0.2)
+            z, best = torch.zeros((n, 64), device="cuda"), torch.zeros(n, **t)
+            K.logit_rules(rows[:, 0], z, best=best, hist=big[:n], hist_len=pos.clamp(max=8), prompt_len=seq, presence=z[:, 0] + 1,
+                          bias_ids=big[:n, :3], bias=torch.ones((n, 8), device="cuda")[:, :3],
+                          mask=big, mask_row=seq)
+            K.check_stream()
+            got.append((k, v, qo, out, z, best))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)

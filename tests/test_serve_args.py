@@ -116,3 +116,30 @@ def test_operators_fail_without_a_device(kq):
         pytest.skip("a GPU is present")
     assert not create(kq)
     assert kq.lib().kq_logit_rules(struct.pack("2P2qP3Pq3P2Pq2Pq6i", *RULES.values()), 0, None) == kq.ERR_BACKEND
+
+
+def test_tensors_of_another_device_are_refused_by_both_ways(kq):
+    """PyTorch tensors take the short way through their DLPack interface; what it cannot take ends in the checks."""
+    torch = pytest.importorskip("torch")
+    from kq import serve
+    z = torch.zeros((2, 64))
+    with pytest.raises(ValueError, match="GPU"):
+        kq.logit_rules(z, z)
+    if getattr(torch.Tensor, "__dlpack_c_exchange_api__", None) is not None:
+        assert serve._Direct.type is torch.Tensor
+        args = [id(z), id(z)] + [None] * 11
+        assert serve._Direct.logit_rules(*args, 0) == serve._Direct.OTHER
+    c = object.__new__(kq.PagedCache)
+    c.h, c.device, c.n_kv, c.page, c.hd, c.type = 1, 0, 2, 16, 64, serve.F16
+    c._free = lambda h: None
+    k, table, i = torch.zeros((1, 2, 64)), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    serve._Direct.page_attend, kept = (lambda *a: serve._Direct.OTHER), serve._Direct.page_attend
+    serve._Direct.page_append, kept2 = (lambda *a: serve._Direct.OTHER), serve._Direct.page_append
+    try:
+        with pytest.raises(ValueError, match="not on device 0"):
+            c.attend(k, table, i, k)
+        with pytest.raises(ValueError, match="not on device 0"):
+            c.append(k, k, table, i)
+    finally:
+        serve._Direct.page_attend, serve._Direct.page_append = kept, kept2
+        c.h = None
