@@ -180,6 +180,19 @@ int kq_batch_caches(kq_model* m, int n_seq);
 int kq_batch_feed(kq_model* m, int seq, const int32_t* toks, int n, int pos);
 int kq_batch_step(kq_model* m, const int32_t* seqs, const int32_t* toks, const int32_t* pos, int n, int32_t* out);
 
+/* Batched decode over a paged cache (whole models; an addition of this library): the sequences share a pool of n_pages
+ * pages of `page` positions per layer and tensor (a power of two from 16 to 1024) instead of owning
+ * ctx positions each, so the memory follows the tokens there are. The caller gives out the pages: row
+ * s of the host page table [n_seq][max_pages] names sequence s's pages in order (a page of a shared
+ * prefix may stand in several rows). kq_paged_caches allocates the pool (zeroed) for tables of up to
+ * max_seq sequences. kq_paged_step runs n <= 128 tokens, token toks[i] at position pos[i] of sequence
+ * seqs[i] attending to [0, pos[i]]: a decode step (one token of each sequence), a prompt chunk
+ * (consecutive positions of one) or both at once; (sequence, position) pairs must be distinct. out null:
+ * the tokens are only fed. Otherwise out[i] gets row i's greedy id under the rules: null (none), or
+ * kq_logit_rules' arguments for n rows (device tensors, ready on `stream`; logits, out, best, n, vocab
+ * and type are the step's own), -1 where a row's rules allow nothing. */
+int kq_paged_caches(kq_model* m, int n_pages, int page, int max_seq);
+
 /* ------------------------------------------------------------------ matrix hooks
  * kc_matvec / kc_dequant equivalents (kcpu4.c:337-341, q4kernels.h:12-36). */
 kq_qmat* kq_qmat_create(int type, int rows, int cols, int device);
@@ -359,6 +372,9 @@ int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table, void* pos
 int kq_page_attend_tensors(kq_pages* c, void* q, void* table, void* len, void* out, void* seq, int window, float scale, void* stream);
 int kq_logit_rules_tensors(void* logits, void* out, void* best, void* hist, void* hist_len, void* prompt_len, void* repetition,
                            void* frequency, void* presence, void* bias_id, void* bias, void* mask, void* mask_row, void* stream);
+
+int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int max_pages, const int32_t* seqs, const int32_t* toks,
+                  const int32_t* pos, int n, const kq_rule_args* rules, void* stream, int32_t* out);
 
 /* Waits for `stream` and reports (and clears) what the operators' kernels flagged on this device. */
 int kq_stream_check(int device, void* stream);

@@ -670,6 +670,15 @@ struct kq_model {
   int* tticket = nullptr;
   size_t tpart_floats = 0;
   int tticket_n = 0;
+  // paged batched decode (kq_paged_caches): one handle per layer over its pool, sharing the first's scratch
+  std::vector<kq_pages*> pages;
+  int pg_n = 0, pg_size = 0, pg_seq = 0;   // pages of the pool, positions of a page, table rows at most
+  float* pqkv = nullptr;            // [MM_MAXM][(nh + 2 nkv) hd] q, k, v rows before the rotation
+  float* patt = nullptr;            // [MM_MAXM][nh hd] attention output
+  float* pscale = nullptr;          // [MM_MAXM] range scales of its packed form
+  float *pcos = nullptr, *psin = nullptr;   // the identity rotation (1, 0): [hd / 2]
+  int *ptable = nullptr, *plen = nullptr, *pzero = nullptr;   // page table, pos + 1, zeros
+  cudaEvent_t pev_in = nullptr;     // the caller's stream up to a step's rules
   bool verify_seq = false;          // node-by-node decode steps instead of the batched pass
   std::vector<void*> allocs;
 };
@@ -862,6 +871,8 @@ static void model_release(kq_model* m) {
   }
   for (kq_qmat* a : {m->emb, m->out})
     if (a) { cudaFree(a->buf); cudaFree(a->tvbuf); delete a; }
+  for (size_t i = m->pages.size(); i-- > 0;) kq_pages_free(m->pages[i]);
+  if (m->pev_in) cudaEventDestroy(m->pev_in);
   for (void* p : m->allocs) cudaFree(p);
   if (m->st_host) cudaFreeHost(m->st_host);
   if (m->vstates) cudaFreeHost(m->vstates);
@@ -2026,8 +2037,10 @@ static bool batch_supported(const kq_model* m) {
 
 // xscale: the per-token scales of the packed input xp (k_bnorm / k_xpack_tok), or null; xsum: its
 // sub-block sums (they enable the exact form for Q4_K row tiles), or null.
+// cos_t, sin_t: rotation tables other than the model's.
 static int launch_tmm(kq_model* m, const SegSpec* ss, int nseg, const __half* xp, const float* xscale,
-                      const float* xsum, int out_ld, const BatchParams& B) {
+                      const float* xsum, int out_ld, const BatchParams& B, const float* cos_t = nullptr,
+                      const float* sin_t = nullptr) {
   prof_mark(m, PC_GEMM);
   TmmParams P;
   tmm_fill(ss, nseg, B.M, m->device, P);
@@ -2036,8 +2049,8 @@ static int launch_tmm(kq_model* m, const SegSpec* ss, int nseg, const __half* xp
   P.xsum = tmm_exact_ok() ? xsum : nullptr;
   P.B = B;
   P.out_ld = out_ld;
-  P.cos_t = m->cos_t;
-  P.sin_t = m->sin_t;
+  P.cos_t = cos_t ? cos_t : m->cos_t;
+  P.sin_t = sin_t ? sin_t : m->sin_t;
   P.hd = m->c.head_dim;
   P.ctx = m->c.ctx;
   P.nkv = m->nkv_l;
@@ -2432,6 +2445,163 @@ extern "C" int kq_batch_step(kq_model* m, const int32_t* seqs, const int32_t* to
   prof_flush(m);
   CU(cudaMemcpy(out, m->out_ids, M * sizeof(int32_t), cudaMemcpyDeviceToHost));
   return check_dev_err(m);
+}
+
+// ------------------------------------------------------------------------------ paged batched decode
+extern "C" int kq_paged_caches(kq_model* m, int n_pages, int page, int max_seq) {
+  int rc = model_check(m);
+  if (rc || (rc = not_tp(m, "kq_paged_caches"))) return rc;
+  if (n_pages < 1 || max_seq < 1 || page < 16 || page > 1024 || (page & (page - 1)))
+    return set_err(KQ_ERR_ARG, "bad page pool (page: a power of two from 16 to 1024)");
+  if (!m->pages.empty())
+    return m->pg_n == n_pages && m->pg_size == page && m->pg_seq == max_seq
+               ? KQ_OK : set_err(KQ_ERR_ARG, "the page pool is already allocated");
+  const kq_config& c = m->c;
+  const size_t per = (size_t)n_pages * m->nkv_l * page * c.head_dim, MM = MM_MAXM;
+  const size_t QD = (size_t)m->nh_l * c.head_dim, KD = (size_t)m->nkv_l * c.head_dim;
+  const int half = c.head_dim / 2;
+  const size_t mark = m->allocs.size();
+  bool ok = true;
+  m->pqkv = dalloc<float>(m, MM * (QD + 2 * KD), ok);
+  m->patt = dalloc<float>(m, MM * QD, ok);
+  m->pscale = dalloc<float>(m, MM, ok);
+  m->pcos = dalloc<float>(m, half, ok);
+  m->psin = dalloc<float>(m, half, ok);
+  m->ptable = dalloc<int>(m, (size_t)max_seq * ((c.ctx + page - 1) / page), ok);
+  m->plen = dalloc<int>(m, MM, ok);
+  m->pzero = dalloc<int>(m, MM, ok);
+  if (ok && !m->bseq) m->bseq = dalloc<int>(m, MM, ok);
+  std::vector<float> one((size_t)half, 1.f);
+  if (ok && cudaMemcpy(m->pcos, one.data(), half * sizeof(float), cudaMemcpyHostToDevice) != cudaSuccess) ok = false;
+  if (ok && !m->pev_in && cudaEventCreateWithFlags(&m->pev_in, cudaEventDisableTiming) != cudaSuccess) ok = false;
+  for (int l = 0; ok && l < c.n_layers; ++l) {
+    kq_page_desc d;
+    std::memset(&d, 0, sizeof(d));
+    d.k = dalloc<__half>(m, per, ok);
+    d.v = dalloc<__half>(m, per, ok);
+    if (!ok) break;
+    d.k_page = d.v_page = (long long)m->nkv_l * page * c.head_dim;
+    d.k_head = d.v_head = (long long)page * c.head_dim;
+    d.k_row = d.v_row = c.head_dim;
+    d.type = KQ_F16; d.n_pages = n_pages; d.page = page; d.n_kv_heads = m->nkv_l; d.head_dim = c.head_dim;
+    kq_pages* p = kqh_pages_create(&d, m->device, l ? m->pages[0] : nullptr);
+    if (p) m->pages.push_back(p);
+    else ok = false;
+  }
+  if (!ok) {   // a server may try again with fewer pages
+    for (size_t i = m->pages.size(); i-- > 0;) kq_pages_free(m->pages[i]);
+    m->pages.clear();
+    while (m->allocs.size() > mark) {
+      if (m->bseq == m->allocs.back()) m->bseq = nullptr;
+      cudaFree(m->allocs.back());
+      m->allocs.pop_back();
+    }
+    cudaGetLastError();
+    return set_err(KQ_ERR_MEMORY, "page pool");
+  }
+  m->pg_n = n_pages;
+  m->pg_size = page;
+  m->pg_seq = max_seq;
+  return KQ_OK;
+}
+
+// A batched pass whose K/V go to pages: the q/k/v GEMM leaves its rows unrotated in fp32 (the rotation
+// epilogue with the identity, which only puts the pairs in place), kq_page_append rotates q and k by the
+// model's tables on the way into the pages, kq_page_attend reads them, and kq_logit_rules picks the ids.
+extern "C" int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int max_pages, const int32_t* seqs, const int32_t* toks,
+                             const int32_t* pos, int n, const kq_rule_args* rules, void* stream, int32_t* out) {
+  int rc = model_check(m);
+  if (rc) return rc;
+  if (m->pages.empty()) return set_err(KQ_ERR_ARG, "kq_paged_caches first");
+  if (!table || !seqs || !toks || !pos || n < 1 || n > MM_MAXM || n_seq < 1 || n_seq > m->pg_seq || max_pages < 1 ||
+      (rules && !out))
+    return set_err(KQ_ERR_ARG, "bad paged step arguments");
+  const kq_config& c = m->c;
+  if ((long long)max_pages > (c.ctx + m->pg_size - 1) / m->pg_size) return set_err(KQ_ERR_ARG, "the page table is wider than the context");
+  for (int i = 0; i < n; ++i) {
+    if (seqs[i] < 0 || seqs[i] >= n_seq) return set_err(KQ_ERR_ARG, "sequence out of range");
+    if (toks[i] < 0 || toks[i] >= c.vocab || pos[i] < 0) return set_err(KQ_ERR_ARG, "Invalid token or position");
+    if (pos[i] >= c.ctx || pos[i] / m->pg_size >= max_pages) return set_err(KQ_ERR_OVERFLOW, "position past the context or its page table");
+    for (int p = 0; p <= pos[i] / m->pg_size; ++p) {
+      const int32_t id = table[(size_t)seqs[i] * max_pages + p];
+      if (id < 0 || id >= m->pg_n) return set_err(KQ_ERR_ARG, "page id out of range");
+    }
+    for (int j = 0; j < i; ++j)
+      if (seqs[j] == seqs[i] && pos[j] == pos[i]) return set_err(KQ_ERR_ARG, "a position occurs twice in a paged step");
+  }
+  if (!batch_supported(m)) return set_err(KQ_ERR_ARG, "configuration not covered by the batched pass");
+  if ((rc = verify_buffers(m)) || (rc = batch_buffers(m))) return rc;
+  cudaStream_t s = m->stream;
+  const int M = n;
+  kq_model::MetaSlot* ms = nullptr;
+  if ((rc = meta_acquire(m, &ms))) return rc;
+  for (int i = 0; i < M; ++i) {
+    ms->tok[i] = toks[i];
+    ms->slot[i] = pos[i];
+    ms->rpos[i] = pos[i] + 1;
+    ms->seq[i] = seqs[i];
+  }
+  CU(cudaMemcpyAsync(m->btok, ms->tok, M * sizeof(int), cudaMemcpyHostToDevice, s));
+  CU(cudaMemcpyAsync(m->bslot, ms->slot, M * sizeof(int), cudaMemcpyHostToDevice, s));
+  CU(cudaMemcpyAsync(m->plen, ms->rpos, M * sizeof(int), cudaMemcpyHostToDevice, s));
+  CU(cudaMemcpyAsync(m->bseq, ms->seq, M * sizeof(int), cudaMemcpyHostToDevice, s));
+  CU(cudaMemcpyAsync(m->ptable, table, (size_t)n_seq * max_pages * sizeof(int), cudaMemcpyHostToDevice, s));
+  if ((rc = meta_release(m))) return rc;
+  BatchParams B;
+  std::memset(&B, 0, sizeof(B));
+  B.M = M; B.rpos = m->pzero;
+  const int hd = c.head_dim, QD = m->nh_l * hd, KD = m->nkv_l * hd, ld = QD + 2 * KD, Npad = (M + 15) & ~15;
+  kq_append_args A;
+  std::memset(&A, 0, sizeof(A));
+  A.q = m->pqkv; A.q_out = m->pqkv; A.k = m->pqkv + QD; A.v = m->pqkv + QD + KD;
+  A.k_tok = A.v_tok = A.q_tok = A.o_tok = ld;
+  A.k_head = A.v_head = A.q_head = A.o_head = hd;
+  A.table = m->ptable; A.seq = m->bseq; A.pos = m->bslot; A.cos_t = m->cos_t; A.sin_t = m->sin_t;
+  A.table_ld = max_pages; A.rope_ld = hd / 2; A.n = M; A.n_heads = m->nh_l; A.src_type = KQ_F32;
+  A.n_seq = n_seq; A.max_pages = max_pages; A.rot = hd; A.n_pos = c.ctx;
+  kq_attend_args T;
+  std::memset(&T, 0, sizeof(T));
+  T.q = m->pqkv; T.out = m->patt; T.q_tok = ld; T.q_head = hd; T.o_tok = QD; T.o_head = hd;
+  T.table = m->ptable; T.seq = m->bseq; T.len = m->plen; T.table_ld = max_pages; T.n = M; T.n_heads = m->nh_l;
+  T.type = KQ_F32; T.n_seq = n_seq; T.max_pages = max_pages; T.scale = (float)(1.0 / std::sqrt((double)hd));
+  for (int l = 0; l < c.n_layers; ++l) {
+    LayerW& w = m->L[l];
+    if ((rc = launch_bnorm(m, M, l == 0, w.attn_norm, l > 0))) return rc;
+    SegSpec qkv[3] = {{w.q, EPI_ROPE_Q, m->pqkv, nullptr}, {w.k, EPI_ROPE_Q, m->pqkv + QD, nullptr}, {w.v, EPI_F32, m->pqkv + QD + KD, nullptr}};
+    if ((rc = launch_tmm(m, qkv, 3, m->bxd, m->bxs_n, m->bxd_sum, ld, B, m->pcos, m->psin))) return rc;
+    prof_mark(m, PC_ATTN);
+    if ((rc = kq_page_append(m->pages[l], &A, s)) || (rc = kq_page_attend(m->pages[l], &T, s))) return rc;
+    prof_mark(m, PC_GEMM);
+    const XPackParams X = {m->patt, QD, QD, Npad, m->bxa, m->pscale, nullptr};
+    CU(launch_pdl(k_xpack_tok, dim3((unsigned)M), dim3(XP_THREADS), 0, s, X));
+    SegSpec so[1] = {{w.o, EPI_F32, m->by, nullptr}};
+    if ((rc = launch_tmm(m, so, 1, m->bxa, m->pscale, nullptr, c.dim, B))) return rc;
+    if ((rc = launch_bnorm(m, M, false, w.ffn_norm, true))) return rc;
+    if ((rc = launch_mlp(m, w, m->by, B))) return rc;
+  }
+  if (out) {
+    if ((rc = launch_bnorm(m, M, false, m->out_norm, true))) return rc;
+    SegSpec sh[1] = {{m->out, EPI_F32, m->vlogits, nullptr}};
+    if ((rc = launch_tmm(m, sh, 1, m->bxd, m->bxs_n, m->bxd_sum, c.vocab, B))) return rc;
+    prof_mark(m, PC_OTHER);
+    kq_rule_args R;
+    if (rules) {
+      R = *rules;
+      CU(cudaEventRecord(m->pev_in, (cudaStream_t)stream));
+      CU(cudaStreamWaitEvent(s, m->pev_in, 0));
+    } else {
+      std::memset(&R, 0, sizeof(R));
+    }
+    R.logits = m->vlogits; R.out = m->vlogits; R.in_ld = R.out_ld = c.vocab; R.best = m->out_ids;
+    R.n = M; R.vocab = c.vocab; R.type = KQ_F32;
+    if ((rc = kq_logit_rules(&R, m->device, s))) return rc;
+  }
+  prof_mark(m, PC_END);
+  if ((rc = tp_sync(m))) return rc;
+  prof_flush(m);
+  if (out) CU(cudaMemcpy(out, m->out_ids, M * sizeof(int32_t), cudaMemcpyDeviceToHost));
+  if ((rc = check_dev_err(m))) return rc;
+  return kq_stream_check(m->device, s);
 }
 
 extern "C" int kq_commit(kq_model* m, const int32_t* path, int k, int pos) {

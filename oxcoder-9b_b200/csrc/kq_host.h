@@ -11,3 +11,8 @@ struct KqhDevice {
 };
 // Initialises `device` on first use, makes it current and describes it; a KQ_* status.
 int kqh_device(int device, KqhDevice* out);
+
+struct kq_pages;
+// kq_pages_create with another handle's attention scratch (null: its own): the handles' calls share a stream,
+// and `with` is freed last.
+kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with);

@@ -29,6 +29,7 @@ struct kq_pages {
   int device = 0, shift = 0;
   KqhDevice dev{};
   AttendScratch scratch{};
+  bool shared = false;   // the scratch belongs to another handle
 };
 
 // The attention kernel of a cache type, head size, query heads per CTA (8 or 16) and precision.
@@ -107,7 +108,8 @@ static int pages_check(const kq_page_desc* d) {
   return KQ_OK;
 }
 
-extern "C" kq_pages* kq_pages_create(const kq_page_desc* given, int device) {
+kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
+  const kq_page_desc* given = static_cast<const kq_page_desc*>(desc);
   KqhDevice dev;
   kq_page_desc own{}, *d = nullptr;
   if (given) {
@@ -129,8 +131,14 @@ extern "C" kq_pages* kq_pages_create(const kq_page_desc* given, int device) {
   c->dev = dev;
   while ((1 << c->shift) < d->page) ++c->shift;
   const size_t part = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
-  cudaError_t e = cudaMalloc(&c->scratch.part, part + PA_MAX_CTAS * sizeof(int));
-  if (e == cudaSuccess) {
+  cudaError_t e = cudaSuccess;
+  if (with) {
+    c->scratch = with->scratch;
+    c->shared = true;
+  } else {
+    e = cudaMalloc(&c->scratch.part, part + PA_MAX_CTAS * sizeof(int));
+  }
+  if (e == cudaSuccess && !with) {
     c->scratch.ticket = reinterpret_cast<int*>(reinterpret_cast<char*>(c->scratch.part) + part);
     e = cudaMemset(c->scratch.ticket, 0, PA_MAX_CTAS * sizeof(int));
   }
@@ -147,9 +155,11 @@ extern "C" kq_pages* kq_pages_create(const kq_page_desc* given, int device) {
   return c;
 }
 
+extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) { return kqh_pages_create(d, device, nullptr); }
+
 extern "C" void kq_pages_free(kq_pages* c) {
   if (!c) return;
-  if (c->scratch.part) {
+  if (c->scratch.part && !c->shared) {
     cudaSetDevice(c->device);
     cudaFree(c->scratch.part);
   }

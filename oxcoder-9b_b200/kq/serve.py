@@ -248,45 +248,10 @@ class PagedCache(object):
         return out
 
 
-def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=None, repetition=None, frequency=None,
-                presence=None, bias_ids=None, bias=None, mask=None, mask_row=None, stream=0):
-    """Penalties for repeated tokens, biases and grammar masks on logits [n, vocab] (fp32, fp16, bf16), into out
-    (may be logits); best [n] int32: the greedy ids (-1 where nothing is allowed). hist [n, most] int32 with
-    hist_len [n] tokens in use, of which prompt_len [n] (None: 0) are the prompt; repetition, frequency, presence:
-    fp32 [n]; bias_ids int32 and bias fp32 [n, entries] (ids outside the vocabulary are padding; the last entry
-    of an id stands); mask int32 or uint32 [masks, >= ceil(vocab / 32)], bit id % 32 of word id / 32 set: allowed;
-    mask_row [n]: a mask for each row, -1 for none (None: mask i for row i)."""
-    T = _Direct.type
-    if type(logits) is not T:
-        _Direct.try_type(type(logits))
-        T = _Direct.type
-    given = (logits, out, best, hist, hist_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, mask_row)
-    if type(logits) is T:
-        ids = []
-        for t in given:
-            if t is None:
-                ids.append(None)
-            elif type(t) is T:
-                ids.append(id(t))
-            else:
-                break
-        else:
-            rc = _Direct.logit_rules(*ids, stream)
-            if not rc:
-                return out
-            if rc != _Direct.OTHER:
-                _bind()[1](rc)
-    shape = logits.shape
-    n, vocab = shape
-    dev, kind = logits.get_device(), _type(logits)
-    if dev < 0:
-        raise ValueError("the logits must be on a GPU")
-    ip, (ild, _) = _rows(logits, "logits", kind, shape, dev)
-    op, (old, _) = _rows(out, "out", kind, shape, dev)
-    if n == 1:
-        ild = old = vocab
+def _rule_fields(n, vocab, dev, hist=None, hist_len=None, prompt_len=None, repetition=None, frequency=None, presence=None,
+                 bias_ids=None, bias=None, mask=None, mask_row=None):
+    """The rules' part of kq_rule_args, checked: 13 pointers and strides, then max_hist, n_bias, n_masks."""
     row = (n,)
-    bp = 0 if best is None else _vec(best, "best", I32, row, dev)
     hp = hl = pl = hld = most = 0
     if hist is not None:
         if hist_len is None:
@@ -331,10 +296,57 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
             mr = _vec(mask_row, "mask_row", I32, row, dev)
     elif mask_row is not None:
         raise ValueError("mask_row without masks")
+    return hp, hl, pl, hld, rp, fp, sp, ap, dp, bld, mp, mr, mld, most, entries, masks
+
+
+def pack_rules(n, vocab, device, **rules):
+    """kq_rule_args of a step that has its own logits (kq_paged_step)."""
+    f = _rule_fields(n, vocab, device, **rules)
+    return _RULES.pack(0, 0, 0, 0, 0, *f[:13], n, vocab, F32, *f[13:])
+
+
+def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=None, repetition=None, frequency=None,
+                presence=None, bias_ids=None, bias=None, mask=None, mask_row=None, stream=0):
+    """Penalties for repeated tokens, biases and grammar masks on logits [n, vocab] (fp32, fp16, bf16), into out
+    (may be logits); best [n] int32: the greedy ids (-1 where nothing is allowed). hist [n, most] int32 with
+    hist_len [n] tokens in use, of which prompt_len [n] (None: 0) are the prompt; repetition, frequency, presence:
+    fp32 [n]; bias_ids int32 and bias fp32 [n, entries] (ids outside the vocabulary are padding; the last entry
+    of an id stands); mask int32 or uint32 [masks, >= ceil(vocab / 32)], bit id % 32 of word id / 32 set: allowed;
+    mask_row [n]: a mask for each row, -1 for none (None: mask i for row i)."""
+    T = _Direct.type
+    if type(logits) is not T:
+        _Direct.try_type(type(logits))
+        T = _Direct.type
+    given = (logits, out, best, hist, hist_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, mask_row)
+    if type(logits) is T:
+        ids = []
+        for t in given:
+            if t is None:
+                ids.append(None)
+            elif type(t) is T:
+                ids.append(id(t))
+            else:
+                break
+        else:
+            rc = _Direct.logit_rules(*ids, stream)
+            if not rc:
+                return out
+            if rc != _Direct.OTHER:
+                _bind()[1](rc)
+    shape = logits.shape
+    n, vocab = shape
+    dev, kind = logits.get_device(), _type(logits)
+    if dev < 0:
+        raise ValueError("the logits must be on a GPU")
+    ip, (ild, _) = _rows(logits, "logits", kind, shape, dev)
+    op, (old, _) = _rows(out, "out", kind, shape, dev)
+    if n == 1:
+        ild = old = vocab
+    bp = 0 if best is None else _vec(best, "best", I32, (n,), dev)
+    fields = _rule_fields(n, vocab, dev, hist, hist_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, mask_row)
     if not n:
         return out
-    rc = _rules()(_RULES.pack(ip, op, ild, old, bp, hp, hl, pl, hld, rp, fp, sp, ap, dp, bld, mp, mr, mld, n, vocab, kind, most,
-                              entries, masks), dev, stream)
+    rc = _rules()(_RULES.pack(ip, op, ild, old, bp, *fields[:13], n, vocab, kind, *fields[13:]), dev, stream)
     if rc:
         _bind()[1](rc)
     return out
