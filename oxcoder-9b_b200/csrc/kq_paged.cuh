@@ -296,14 +296,17 @@ struct PaShape {
   static constexpr int KV = 2 * PA_SUB * LD;                   // K and V rows of one step of a warp
   static constexpr int QX = HEADS * (HD + 8) * 4;              // a segment's query rows, or a warp's (o, m, l) rows
   static constexpr int STAGE = KV > QX ? KV : QX;              // a ring slot holds any of the three
-  static constexpr int FIT = 104 * 1024 / (PA_WARPS * STAGE);
-  static constexpr int STAGES = FIT < 3 ? 3 : FIT > 8 ? 8 : FIT;   // two CTAs per SM where three stages leave the room
   static constexpr int KS = HD / 16;
   static constexpr int NQ = PREC ? (BF ? 3 : 2) : 1;           // terms of a query element
   static constexpr int NP = PREC ? (BF ? 3 : 2) : 2;           // terms of a softmax weight
   static constexpr bool QREG = KS * NQ * NT * 2 <= 64;         // query fragments in registers, else in shared memory
   static constexpr int QBYTES = QREG ? 0 : KS * NQ * NT * 256;
   static constexpr int MLD = HD + 4;                           // row of the warps' exchange: o, m, l
+  // CTAs per SM: three of shallower rings measured slower (one 4K sequence 15.4 against 13.5 us, 64 x 32K 845 against 809)
+  static constexpr int PER_SM = STAGE > 12000 ? 1 : 2;
+  static constexpr int FIT = (226 * 1024 / PER_SM - 4608 - QBYTES) / (PA_WARPS * STAGE);
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static_assert(STAGES >= 2, "a ring of two slots at least");
   static constexpr int SMEM = PA_WARPS * STAGES * STAGE + QBYTES;
 };
 constexpr int PA_JOIN = 16;                    // partials of a chain read at once
@@ -336,7 +339,7 @@ struct PaCursor {
 // written out; otherwise its (o, m, l) goes to the scratch and the last CTA of the chain to arrive
 // joins the chain's partials in CTA order, so the sums' order is fixed.
 template <int CT, int HD, int NT, bool PREC>
-__global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
+__global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_SM) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
   using S = PaShape<CT, HD, NT, PREC>;
   constexpr bool BF = S::BF, E8 = CT == PG_E4M3;
   constexpr int KS = S::KS, NQ = S::NQ, NP = S::NP;
@@ -345,6 +348,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   __shared__ __align__(16) float4 s_sum[PA_WARPS * 32];
   __shared__ float2 s_ml[PA_WARPS * 32];
   __shared__ long long s_start;
+  __shared__ KeyRange s_keys;
+  __shared__ int s_tiles;
   __shared__ long long s_scan[PA_WARPS];
   __shared__ int s_seq, s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, t4 = lane & 3;
@@ -388,10 +393,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   if (begin < end && before * H <= begin && begin < (before + mine) * H) {
     long long b = before;
     for (int i = i0; i < i1; ++i) {
-      const int u = units_of(i);
+      KeyRange R;
+      const int t = tiles_of(i, R), u = t ? t + PA_COST : 0;
       if (begin < (b + u) * H) {
         s_seq = i;
         s_start = b * H;
+        s_keys = R;
+        s_tiles = t;
         break;
       }
       b += u;
@@ -424,7 +432,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   };
   PaCursor cur;
   cur.seq = s_seq;
-  cur.tiles = tiles_of(cur.seq, cur.R);
+  cur.tiles = s_tiles;
+  cur.R = s_keys;
   cur.head = (int)pa_div(begin - s_start, cur.tiles + PA_COST);
   cur.seg = s_start + (long long)cur.head * (cur.tiles + PA_COST);
   cur.at = (int)(begin - cur.seg);
@@ -442,10 +451,15 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
   uint32_t pages_ok = 0;                               // one bit per slot: its page exists
   int slot = 0, fill = 0;
   // of the loader's segment: this lane's place in row 0 of its head, the table row; and of the next step
-  // its first key and page id (requested a step ahead, so that no copy waits for the table)
+  // its first key; and the page ids of 32 steps, a lane each, requested together when the segment begins:
+  // no copy waits for the table on its own
   const char *kseg = nullptr, *vseg = nullptr;
   const int* tseg = nullptr;
-  int ld_key = 0, ld_page = -1;
+  int ld_key = 0, ld_pages = -1;
+  auto request_pages = [&]() {   // of the steps from the current one on
+    const int t = max(ld_tile, ld.t0) + lane, key = (ld.R.first & ~(PA_SUB - 1)) + t * PA_TILE + warp * PA_SUB;
+    ld_pages = t < ld.t1 && key < ld.R.last ? tseg[key >> P.T.page_shift] : -1;
+  };
   auto begin_segment = [&]() {
     const int kv = ld.head / HT;
     kseg = reinterpret_cast<const char*>(P.kc) + (kv * P.kh + lr * P.kr) * S::ES + lc * 16;
@@ -453,6 +467,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
     tseg = P.T.table + ld.R.row * P.T.ld;
     ld_key = (ld.R.first & ~(PA_SUB - 1)) + ld.t0 * PA_TILE + warp * PA_SUB;
     ld_tile = ld.t0 - 1;
+    request_pages();
   };
   if (ld.left > 0) begin_segment();
   auto load = [&]() {
@@ -467,6 +482,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
           pa_cp16(dst + h * q_ld + c * 16, q + h * P.q_head * q_es + c * 16, 16u);
         }
       } else {
+        const int step_of = ld_tile - ld.t0;
+        if (step_of > 0 && (step_of & 31) == 0) request_pages();
+        const int ld_page = __shfl_sync(0xffffffffu, ld_pages, step_of & 31);
         if (ld_key < ld.R.last) {
           const bool ok = ld_page >= 0 && ld_page < P.T.n_pages;
           pages_ok = (pages_ok & ~(1u << fill)) | ((uint32_t)ok << fill);
@@ -497,7 +515,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) k_page_attend(const __grid_c
         next_segment(ld);
         if (ld.left > 0) begin_segment();
       }
-      if (ld.left > 0 && ld_key < ld.R.last) ld_page = tseg[ld_key >> P.T.page_shift];
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;

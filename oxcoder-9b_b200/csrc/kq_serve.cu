@@ -36,11 +36,11 @@ struct kq_pages {
 typedef void (*AttendFn)(AttendParams, AttendScratch);
 struct AttendKernel {
   AttendFn fn;
-  int smem;
+  int smem, per_sm;
 };
 template <int CT, int HD, int NT, bool PREC>
 static AttendKernel attend_entry() {
-  return {k_page_attend<CT, HD, NT, PREC>, PaShape<CT, HD, NT, PREC>::SMEM};
+  return {k_page_attend<CT, HD, NT, PREC>, PaShape<CT, HD, NT, PREC>::SMEM, PaShape<CT, HD, NT, PREC>::PER_SM};
 }
 template <int CT, int HD>
 static AttendKernel attend_of(bool wide, bool prec) {
@@ -246,8 +246,7 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* st
   const int heads = G > 8 ? 16 : 8;
   const long long tiles = (((long long)a->max_pages << c->shift) + PA_TILE - 1) / PA_TILE;
   const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
-  const int per_sm = k.smem > 110 * 1024 ? 1 : 2;
-  const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * per_sm));
+  const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * k.per_sm));
   CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, 1, P, c->scratch));
   return KQ_OK;
 }
