@@ -56,21 +56,19 @@ struct AppendParams {
   int* err;
 };
 
-// V consecutive elements of type T (16 bytes of fp32 or 16-bit elements) as fp32.
+// 16 bytes of elements of type T as V values.
 template <int T, int V>
-__device__ __forceinline__ void ap_load(const void* p, float (&x)[V]) {
-  if (T == PG_F32) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void ap_widen(const uint4& a, float (&x)[V]) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {
+    if (T == PG_F32) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
       const float2 f = T == PG_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
                                    : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+      x[(2 * i) % V] = f.x;
+      x[(2 * i + 1) % V] = f.y;
     }
   }
 }
@@ -105,84 +103,97 @@ __device__ __forceinline__ void ap_store(void* p, const float (&x)[V]) {
 }
 
 // Bound by memory: each source row is read and each stored row written once, in 16-byte loads. Grid
-// (token, slice of its head rows); a thread owns V pairs (j, j + rot / 2) of one head row, V = 16 bytes
-// of the source type, or 2 V dims that do not turn. The row's loads do not wait for the position;
-// the position, the table entry and the angles follow one another.
+// (token, slice of its head rows); a thread owns V pairs (j, j + rot / 2), V = 16 bytes of the source type, or 2 V
+// dims that do not turn, of U head rows: the rows' loads are all requested before the position is known,
+// and one look at the table and the angles serves them all.
 constexpr int AP_THREADS = 128;
-template <int ST, int CT>
+constexpr int AP_DEEP = 3;   // head rows per thread of a large append
+template <int ST, int CT, int U>
 __global__ void __launch_bounds__(AP_THREADS) k_page_append(const __grid_constant__ AppendParams P) {
   constexpr int V = ST == PG_F32 ? 4 : 8, ES = ST == PG_F32 ? 4 : 2, CS = CT == PG_E4M3 ? 1 : 2;
   pdl_wait();
   pdl_trigger();
-  const int i = blockIdx.x, units = P.hd / (2 * V), e = blockIdx.y * AP_THREADS + threadIdx.x;
-  const int r = e / units, u = e % units;
-  if (r >= P.n_heads + 2 * P.n_kv) return;
+  const int i = blockIdx.x, units = P.hd / (2 * V), u = threadIdx.x % units;   // units divides AP_THREADS
+  const int r0 = (blockIdx.y * U * AP_THREADS + threadIdx.x) / units, rstep = AP_THREADS / units;
+  const int rows = P.n_heads + 2 * P.n_kv, half = P.rot / 2;
+  const int jt = u < half / V ? u * V : 2 * V * u, jt2 = u < half / V ? jt + half : jt + V;   // rows that turn
   const int pos = P.pos[i];
-  const bool is_q = r < P.n_heads, is_v = r >= P.n_heads + P.n_kv;
-  const int h = is_q ? r : is_v ? r - P.n_heads - P.n_kv : r - P.n_heads;
-  const int half = is_v ? 0 : P.rot / 2;
-  const bool turn = u < half / V;
-  const int j = turn ? u * V : 2 * V * u, j2 = turn ? j + half : j + V;   // the thread's two runs of V dims
-  const char* src = reinterpret_cast<const char*>(is_q ? P.q : is_v ? P.v : P.k) +
-                    (is_q ? i * P.q_tok + h * P.q_head : is_v ? i * P.v_tok + h * P.v_head : i * P.k_tok + h * P.k_head) * ES;
-  float a[V], b[V];
-  ap_load<ST, V>(src + j * ES, a);
-  ap_load<ST, V>(src + j2 * ES, b);
+  uint4 ra[U], rb[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int r = r0 + k * rstep;
+    if (r < rows) {
+      const bool is_q = r < P.n_heads, is_v = r >= P.n_heads + P.n_kv;
+      const int h = is_q ? r : is_v ? r - P.n_heads - P.n_kv : r - P.n_heads;
+      const char* src = reinterpret_cast<const char*>(is_q ? P.q : is_v ? P.v : P.k) +
+                        (is_q ? i * P.q_tok + h * P.q_head : is_v ? i * P.v_tok + h * P.v_head : i * P.k_tok + h * P.k_head) * ES;
+      ra[k] = *reinterpret_cast<const uint4*>(src + (is_v ? 2 * V * u : jt) * ES);
+      rb[k] = *reinterpret_cast<const uint4*>(src + (is_v ? 2 * V * u + V : jt2) * ES);
+    }
+  }
   if (pos < 0) return;
   if (P.rot && pos >= P.n_pos) {
     atomicOr(P.err, KQ_DEV_ERR_BAD_POS);
     return;
   }
-  long long page = 0;
-  float scale = 1.f;
-  if (!is_q) {
-    const int s = P.T.seq ? P.T.seq[i] : i, pi = pos >> P.T.page_shift;
-    if (s < 0 || s >= P.T.n_seq || pi >= P.T.max_pages) {
-      atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW : KQ_DEV_ERR_BAD_POS);
-      return;
-    }
-    page = P.T.table[s * P.T.ld + pi];
-    if (page < 0 || page >= P.T.n_pages) {
-      atomicOr(P.err, KQ_DEV_ERR_BAD_PAGE);
-      return;
-    }
-    const float* sc = is_v ? P.vs : P.ks;
-    if (CT == PG_E4M3 && sc) scale = sc[h];
-  }
-  if (turn) {
-    float c[V], s[V];
+  // the page; a bad one keeps the keys and values out, the queries are still turned
+  const int s = P.T.seq ? P.T.seq[i] : i, pi = pos >> P.T.page_shift;
+  long long page = -1;
+  if (s >= 0 && s < P.T.n_seq && pi < P.T.max_pages) page = P.T.table[s * P.T.ld + pi];
+  float c[V], sn[V];
+  if (u < half / V) {
 #pragma unroll
     for (int x = 0; x < V; x += 4) {
-      const float4 cc = *reinterpret_cast<const float4*>(P.cos_t + pos * P.rope_ld + j + x);
-      const float4 ss = *reinterpret_cast<const float4*>(P.sin_t + pos * P.rope_ld + j + x);
+      const float4 cc = *reinterpret_cast<const float4*>(P.cos_t + pos * P.rope_ld + jt + x);
+      const float4 ss = *reinterpret_cast<const float4*>(P.sin_t + pos * P.rope_ld + jt + x);
       c[x] = cc.x; c[x + 1] = cc.y; c[x + 2] = cc.z; c[x + 3] = cc.w;
-      s[x] = ss.x; s[x + 1] = ss.y; s[x + 2] = ss.z; s[x + 3] = ss.w;
-    }
-#pragma unroll
-    for (int x = 0; x < V; ++x) {
-      const float p = a[x], q = b[x];
-      a[x] = __fsub_rn(__fmul_rn(p, c[x]), __fmul_rn(q, s[x]));
-      b[x] = __fadd_rn(__fmul_rn(q, c[x]), __fmul_rn(p, s[x]));
+      sn[x] = ss.x; sn[x + 1] = ss.y; sn[x + 2] = ss.z; sn[x + 3] = ss.w;
     }
   }
-  if (is_q) {
-    char* dst = reinterpret_cast<char*>(P.q_out) + (i * P.o_tok + h * P.o_head) * ES;
-    ap_store<ST, V>(dst + j * ES, a);
-    ap_store<ST, V>(dst + j2 * ES, b);
-    return;
-  }
-  if (CT == PG_E4M3) {
-#pragma unroll
-    for (int x = 0; x < V; ++x) {
-      a[x] = __fdiv_rn(a[x], scale);
-      b[x] = __fdiv_rn(b[x], scale);
-    }
+  if (page < 0 || page >= P.T.n_pages) {
+    if (r0 + (U - 1) * rstep >= P.n_heads)
+      atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW : pi >= P.T.max_pages ? KQ_DEV_ERR_BAD_POS : KQ_DEV_ERR_BAD_PAGE);
+    page = -1;
   }
   const int row = pos & ((1 << P.T.page_shift) - 1);
-  char* dst = reinterpret_cast<char*>(is_v ? P.vc : P.kc) +
-              (is_v ? page * P.vp + h * P.vh + row * P.vr : page * P.kp + h * P.kh + row * P.kr) * CS;
-  ap_store<CT, V>(dst + j * CS, a);
-  ap_store<CT, V>(dst + j2 * CS, b);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int r = r0 + k * rstep;
+    if (r >= rows) break;
+    const bool is_q = r < P.n_heads, is_v = r >= P.n_heads + P.n_kv;
+    const int h = is_q ? r : is_v ? r - P.n_heads - P.n_kv : r - P.n_heads;
+    const int j = is_v ? 2 * V * u : jt, j2 = is_v ? j + V : jt2;
+    float a[V], b[V];
+    ap_widen<ST, V>(ra[k], a);
+    ap_widen<ST, V>(rb[k], b);
+    if (!is_v && u < half / V) {
+#pragma unroll
+      for (int x = 0; x < V; ++x) {
+        const float p = a[x], q = b[x];
+        a[x] = __fsub_rn(__fmul_rn(p, c[x]), __fmul_rn(q, sn[x]));
+        b[x] = __fadd_rn(__fmul_rn(q, c[x]), __fmul_rn(p, sn[x]));
+      }
+    }
+    if (is_q) {
+      char* dst = reinterpret_cast<char*>(P.q_out) + (i * P.o_tok + h * P.o_head) * ES;
+      ap_store<ST, V>(dst + j * ES, a);
+      ap_store<ST, V>(dst + j2 * ES, b);
+    } else if (page >= 0) {
+      if (CT == PG_E4M3) {
+        const float* sc = is_v ? P.vs : P.ks;
+        const float scale = sc ? sc[h] : 1.f;
+#pragma unroll
+        for (int x = 0; x < V; ++x) {
+          a[x] = __fdiv_rn(a[x], scale);
+          b[x] = __fdiv_rn(b[x], scale);
+        }
+      }
+      char* dst = reinterpret_cast<char*>(is_v ? P.vc : P.kc) +
+                  (is_v ? page * P.vp + h * P.vh + row * P.vr : page * P.kp + h * P.kh + row * P.kr) * CS;
+      ap_store<CT, V>(dst + j * CS, a);
+      ap_store<CT, V>(dst + j2 * CS, b);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------ attention
@@ -250,6 +261,12 @@ __device__ __forceinline__ uint32_t pa_trans(uint32_t a) {
 }
 __device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 2^x to 2 ulp (the instruction's documented error); results below 2^-126 are 0.
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // Two e4m3 bytes (the low half of x) as fp16; exact.
 __device__ __forceinline__ uint32_t pa_e4m3x2(uint32_t x) {
@@ -655,10 +672,10 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const float mn = fmaxf(m[nt][c], mx), u = mn == -INFINITY ? 0.f : mn;
-          f[nt][c] = exp2f(m[nt][c] - u);
+          f[nt][c] = pa_exp2(m[nt][c] - u);
           m[nt][c] = mn;
-          x[c] = exp2f(x[c] - u) * PSCALE;
-          x[c + 2] = exp2f(x[c + 2] - u) * PSCALE;
+          x[c] = pa_exp2(x[c] - u) * PSCALE;
+          x[c + 2] = pa_exp2(x[c + 2] - u) * PSCALE;
           l[nt][c] = __fmaf_rn(l[nt][c], f[nt][c], x[c] + x[c + 2]);
         }
         uint32_t ta[NP], tb[NP];
@@ -744,7 +761,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) {
         const float* row = xrow(w, h);
-        const float wt = exp2f(row[HD] - u);
+        const float wt = pa_exp2(row[HD] - u);
         L = __fmaf_rn(wt, row[HD + 1], L);
         O = __fmaf_rn(wt, row[d], O);
       }
@@ -791,13 +808,13 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
             }
 #pragma unroll
             for (int j = 0; j < PA_JOIN; ++j) mx = fmaxf(mx, s2[j].x);
-            const float u = mx == -INFINITY ? 0.f : mx, f = exp2f(M - u);
+            const float u = mx == -INFINITY ? 0.f : mx, f = pa_exp2(M - u);
             M = mx;
             L *= f;
             O.x *= f; O.y *= f; O.z *= f; O.w *= f;
 #pragma unroll
             for (int j = 0; j < PA_JOIN; ++j) {
-              const float wt = exp2f(s2[j].x - u);
+              const float wt = pa_exp2(s2[j].x - u);
               L = __fmaf_rn(wt, s2[j].y, L);
               O.x = __fmaf_rn(wt, v[j].x, O.x); O.y = __fmaf_rn(wt, v[j].y, O.y);
               O.z = __fmaf_rn(wt, v[j].z, O.z); O.w = __fmaf_rn(wt, v[j].w, O.w);
@@ -827,7 +844,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
             for (int x = 1; x < groups; ++x) {
               const float4 v = s_sum[x * cols + e];
               const float2 s2 = s_ml[x * cols + e];
-              const float mx = fmaxf(M, s2.x), u = mx == -INFINITY ? 0.f : mx, f = exp2f(M - u), wt = exp2f(s2.x - u);
+              const float mx = fmaxf(M, s2.x), u = mx == -INFINITY ? 0.f : mx, f = pa_exp2(M - u), wt = pa_exp2(s2.x - u);
               M = mx;
               L = __fmaf_rn(wt, s2.y, L * f);
               O.x = __fmaf_rn(wt, v.x, O.x * f); O.y = __fmaf_rn(wt, v.y, O.y * f);

@@ -95,6 +95,8 @@ def within(got, want, err, kind):
     ("float32", "bfloat16", 64, 12, 12, 16, 16, 50, 7, True),
     ("float32", "float8_e4m3fn", 64, 1, 1, 16, 64, 3, 1, False),
     ("float16", "bfloat16", 128, 2, 2, 32, 0, 21, 5, False),
+    ("float32", "float16", 128, 2, 6, 16, 64, 5000, 25, False),
+    ("bfloat16", "float8_e4m3fn", 128, 8, 17, 16, 128, 5000, 25, True),
 ])
 def test_append(env, src, cache, hd, kv, heads, page, rot, n, seqs, token_major):
     K, torch = env
