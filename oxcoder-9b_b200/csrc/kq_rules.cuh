@@ -91,12 +91,11 @@ template <> struct RlCount<true> { using type = uint32_t; static constexpr uint3
 // shares gave one CTA of each row most of the touched ids). First the CTA counts its ids' occurrences in shared memory: a short history is
 // scanned by every CTA of the row (16 KB from the L2 each, no barrier between CTAs), a long one (over
 // RL_LOCAL) by its parts, with the hits sent to the owner's shared memory. The first to count an id
-// lists it, and the listed ids are handled next, a thread each. Then the rest streams through registers,
-// RL_BATCH groups of 16 bytes a thread ahead (the first batch flies during the scan): mask, write, pick.
-// (Touched ids handled within the stream cost every warp their whole latency at almost every step: 128
-// rows with up to 4096 tokens took 124 us; a thread for each token, the first to take an id handling it,
-// 64 to 72.) Counts are integer adds and the last bias entry is a maximum, so nothing depends on the
-// order of arrival.
+// lists it. Then the CTA's logits stream through registers, RL_BATCH groups of 16 bytes a thread ahead (the
+// first batch flies during the scan): mask, write, pick among the untouched; and last the listed ids, a
+// thread each. (Touched ids handled within the stream cost every warp their whole latency at almost every
+// step: 128 rows with up to 4096 tokens took 124 us.) Counts are integer adds and the last bias entry is
+// a maximum, so nothing depends on the order of arrival.
 // Positions count from the 16-byte boundary at or below the row's start (u = id + shift), so rows of
 // any alignment move in 16-byte groups; only the groups over a row's ends are handled element by element.
 template <typename T, bool LONG>
@@ -110,11 +109,6 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   const int tid = threadIdx.x, rank = (int)rl_rank(), ranks = (int)rl_ranks(), i = blockIdx.x / ranks, span = P.span;
   Count* cnt = reinterpret_cast<Count*>(rl_smem);                                    // [span]
   const bool counted = P.hist || P.n_bias;
-  if (counted)
-    for (int j = tid; j < span * (int)sizeof(Count) / 16; j += RL_THREADS) reinterpret_cast<uint4*>(cnt)[j] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) s_entries = s_n = 0;
-  pdl_wait();
-  pdl_trigger();
   const T* in = reinterpret_cast<const T*>(P.in) + i * P.in_ld;
   T* out = reinterpret_cast<T*>(P.out) + i * P.out_ld;
   const int shift = (int)((reinterpret_cast<uintptr_t>(in) / sizeof(T)) % VEC);
@@ -125,16 +119,30 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   auto owner = [&](int u) { return (u / STEP) & (ranks - 1); };
   auto local = [&](int u) { return ((u / STEP) >> lg) * STEP + (u & (STEP - 1)); };
   auto place = [&](int turn) { return (turn * ranks + rank) * STEP; };   // where this CTA's turn begins
-  auto whole = [&](int u) { return u >= shift && u + VEC <= u_end; };
+  // the CTA's logits on their way from memory to the L2 while it counts (whole groups, a thread per turn; the
+  // L2 is where writes of the kernel before this one arrive too, so this need not wait for it)
+  if (counted && place(tid) < u_end) {
+    const int a = max(place(tid), shift ? VEC : 0), b = min(place(tid) + STEP, u_end / VEC * VEC);
+    if (a < b)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(in + (a - shift)), "r"((b - a) * (int)sizeof(T)) : "memory");
+  }
+  if (counted)
+    for (int j = tid; j < span * (int)sizeof(Count) / 16; j += RL_THREADS) reinterpret_cast<uint4*>(cnt)[j] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) s_entries = s_n = 0;
+  pdl_wait();
+  pdl_trigger();
+  // turns [t_lo, t_hi) lie inside the row, both rows aligned alike: whole groups, no checks
+  const int turns = u_end > rank * STEP ? (u_end - rank * STEP - 1) / (ranks * STEP) + 1 : 0;
+  const int t_lo = rank == 0 && shift ? 1 : 0;
+  const int t_hi = vec_out ? max(t_lo, (u_end - rank * STEP) / STEP > 0 ? ((u_end - rank * STEP) / STEP - 1) / ranks + 1 : 0) : t_lo;
+  const int first = tid * VEC - shift;                                   // id of this thread's group in the turn at 0
   uint4 x[RL_BATCH];
   auto request = [&](int turn) {
 #pragma unroll
-    for (int k = 0; k < RL_BATCH; ++k) {
-      const int u = place(turn + k) + tid * VEC;
-      if (whole(u)) x[k] = *reinterpret_cast<const uint4*>(in + (u - shift));
-    }
+    for (int k = 0; k < RL_BATCH; ++k)
+      if (turn + k < t_hi) x[k] = *reinterpret_cast<const uint4*>(in + (place(turn + k) + first));
   };
-  request(0);
+  request(t_lo);
   const int nh = P.hist ? min(max(P.hist_len[i], 0), P.max_hist) : 0;
   const int np = P.prompt_len ? P.prompt_len[i] : 0;
   int mrow = P.mask ? (P.mask_row ? P.mask_row[i] : i) : -1;
@@ -150,12 +158,10 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   uint32_t m[RL_BATCH];                                   // the mask word of a group's first id
   auto request_mask = [&](int turn) {
 #pragma unroll
-    for (int k = 0; k < RL_BATCH; ++k) {
-      const int u = place(turn + k) + tid * VEC;
-      m[k] = mask && u < u_end ? mask[max(u - shift, 0) >> 5] : 0xffffffffu;
-    }
+    for (int k = 0; k < RL_BATCH; ++k)
+      if (mask && turn + k < t_hi) m[k] = mask[(place(turn + k) + first) >> 5];
   };
-  request_mask(0);
+  request_mask(t_lo);
   float bv = -INFINITY;
   int bi = 0x7fffffff;
   auto better = [&](float v, int j) {                     // equal values: the lowest id
@@ -163,8 +169,8 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   };
   auto mine = [&](int id) { return id >= 0 && id < P.vocab && owner(id + shift) == rank; };
   auto mask_of = [&](int id) { return mask ? mask[id >> 5] : 0xffffffffu; };
+  const bool apart = nh > RL_LOCAL;                       // the same for all CTAs of the row
   if (counted) {
-    const bool apart = nh > RL_LOCAL;                     // the same for all CTAs of the row
     if (apart) rl_cluster_sync();                         // every CTA's counts are zero
     else __syncthreads();
     // adds to, or sets bits of, the count of one of this CTA's ids (h < 0: none), and lists it if it was 0; whole warps
@@ -219,7 +225,100 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
     }
     if (apart) rl_cluster_sync();                         // every hit has arrived
     else __syncthreads();
+  }
+
+  // ---- the stream: masks and writes every id, picks among the untouched. It keeps its largest value and
+  // that value's turn; the id is looked up once, at the end.
+  float top = -INFINITY;
+  int top_turn = -1;
+  constexpr int CW = VEC * (int)sizeof(Count) / 4;
+  auto fast = [&](int turn, const uint4& v, uint32_t w) {
+    union { uint4 q; T t[VEC]; } y;
+    y.q = v;
+    const int id = place(turn) + first;
+    if (mask) {                                           // bit j: id + j is allowed
+      uint32_t next = 0;
+      if (shift && (id & 31) + VEC > 32 && (id >> 5) + 1 < (P.vocab + 31) >> 5) next = mask[(id >> 5) + 1];
+      w = __funnelshift_r(w, next, id & 31);
+    }
+    if (mask || none) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (none || !((w >> j) & 1u)) y.t[j] = rl_put<T>(-INFINITY);
+    }
+    *reinterpret_cast<uint4*>(out + id) = y.q;
+    uint32_t c[CW], any = 0;                              // the group's counts
+    if (counted) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) {
+        const uint2 t = reinterpret_cast<const uint2*>(cnt + turn * STEP + tid * VEC)[j / 2];
+        c[j] = t.x;
+        c[j + 1] = t.y;
+        any |= t.x | t.y;
+      }
+    }
+    float most = -INFINITY;
+    if (!any) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) most = fmaxf(most, rl_get<T>(y.t[j]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (LONG ? c[j] == 0 : ((c[j / 2] >> (16 * (j & 1))) & 0xffffu) == 0) most = fmaxf(most, rl_get<T>(y.t[j]));
+    }
+    if (most > top) {
+      top = most;
+      top_turn = turn;
+    }
+  };
+  auto edge = [&](int turn) {                             // a turn over an end of the row, or unlike alignments
+    const int id0 = place(turn) + first;
+    if (vec_out && id0 >= 0 && id0 + VEC <= P.vocab) {
+      fast(turn, *reinterpret_cast<const uint4*>(in + id0), mask ? mask[id0 >> 5] : 0u);
+      return;
+    }
+#pragma unroll 1
+    for (int j = 0; j < VEC; ++j) {
+      const int id = id0 + j;
+      if (id < 0 || id >= P.vocab) continue;
+      const bool allowed = !none && (!mask || ((mask[id >> 5] >> (id & 31)) & 1u));
+      const T r = allowed ? in[id] : rl_put<T>(-INFINITY);
+      out[id] = r;
+      const float f = rl_get<T>(r);
+      if (f > -INFINITY && !(counted && cnt[turn * STEP + tid * VEC + j])) better(f, id);
+    }
+  };
+  // turns in their order: of equal values a thread keeps the first
+#pragma unroll 1
+  for (int turn = 0; turn < min(t_lo, turns); ++turn) edge(turn);
+#pragma unroll 1
+  for (int turn = t_lo; turn < t_hi; turn += RL_BATCH) {
+    uint4 v[RL_BATCH];
+    uint32_t w[RL_BATCH];
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k) {
+      v[k] = x[k];
+      w[k] = m[k];
+    }
+    request(turn + RL_BATCH);
+    request_mask(turn + RL_BATCH);
+#pragma unroll
+    for (int k = 0; k < RL_BATCH; ++k)
+      if (turn + k < t_hi) fast(turn + k, v[k], w[k]);
+  }
+#pragma unroll 1
+  for (int turn = t_hi; turn < turns; ++turn) edge(turn);
+  if (top_turn >= 0) {
+    for (int j = VEC - 1; j >= 0; --j) {                  // the lowest of the group's untouched ids with that value
+      const int id = place(top_turn) + first + j;
+      if (!(counted && cnt[top_turn * STEP + tid * VEC + j]) && rl_get<T>(out[id]) == top) better(top, id);
+    }
+  }
+
+  if (counted) {
+    __syncthreads();                                      // the stream has written the touched ids too
     const int entries = s_entries;
+    // v: the id's logit (in place: the value itself, or masked and about to be again)
     auto apply = [&](int h, uint32_t c, float v, uint32_t word) {
       if (c & ~K::BIASED) v = rl_penalise(v, (c & K::MOST) | ((c & K::PROMPT) ? 0x80000000u : 0u), rep, freq, pres);
       if (c & K::BIASED) {                                // the last entry of the list with this id
@@ -254,61 +353,6 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
         if (cnt[at]) apply(h, cnt[at], rl_get<T>(in[h]), mask_of(h));
       }
     }
-  }
-
-  auto stream = [&](int u, const uint4& v, uint32_t w) {
-    if (u >= u_end) return;
-    const int id0 = u - shift;                            // below 0 only in a row's first group
-    constexpr int CW = VEC * (int)sizeof(Count) / 4;
-    uint32_t c[CW], any = 0;                              // the group's counts
-#pragma unroll
-    for (int j = 0; j < CW; ++j) c[j] = 0;
-    if (counted) {
-#pragma unroll
-      for (int j = 0; j < CW; j += 2) {
-        const uint2 t = reinterpret_cast<const uint2*>(cnt + local(u))[j / 2];
-        c[j] = t.x;
-        c[j + 1] = t.y;
-        any |= t.x | t.y;
-      }
-    }
-    if (mask) {                                           // bit j: id0 + j is allowed
-      const int e0 = max(id0, 0), s = e0 & 31;
-      uint32_t next = 0;
-      if (s + VEC > 32 && (e0 >> 5) + 1 < (P.vocab + 31) >> 5) next = mask[(e0 >> 5) + 1];
-      w = __funnelshift_r(w, next, s) << (id0 < 0 ? -id0 : 0);
-    }
-    if (none) w = 0;
-    const bool all = whole(u), plain = all && vec_out && !any;
-    union { uint4 q; T t[VEC]; } y;
-    y.q = v;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (!all) {
-        if (id0 + j < 0 || u + j >= u_end) continue;
-        y.t[j] = in[id0 + j];
-      }
-      if (!((w >> j) & 1u)) y.t[j] = rl_put<T>(-INFINITY);
-      const float f = rl_get<T>(y.t[j]);
-      const bool clear = LONG ? c[j] == 0 : ((c[j / 2] >> (16 * (j & 1))) & 0xffffu) == 0;
-      if (!plain && clear) out[id0 + j] = y.t[j];         // the touched ids are written already
-      if (clear && f > -INFINITY) better(f, id0 + j);
-    }
-    if (plain) *reinterpret_cast<uint4*>(out + id0) = y.q;
-  };
-#pragma unroll 1
-  for (int turn = 0; place(turn) < u_end; turn += RL_BATCH) {
-    uint4 v[RL_BATCH];
-    uint32_t w[RL_BATCH];
-#pragma unroll
-    for (int k = 0; k < RL_BATCH; ++k) {
-      v[k] = x[k];
-      w[k] = m[k];
-    }
-    request(turn + RL_BATCH);
-    request_mask(turn + RL_BATCH);
-#pragma unroll
-    for (int k = 0; k < RL_BATCH; ++k) stream(place(turn + k) + tid * VEC, v[k], w[k]);
   }
   if (!P.best) return;
   // ---- the greedy id: warp, CTA, cluster
