@@ -76,7 +76,7 @@ __device__ __forceinline__ void rl_max(uint32_t a, uint32_t v) {
 constexpr int RL_THREADS = 512;
 constexpr int RL_CLUSTER = 16;       // CTAs of a row at most
 constexpr int RL_BYTES = 76 * 1024;  // of counts a CTA holds at most if it may: two CTAs per SM
-constexpr int RL_BATCH = 4;          // 16-byte groups of logits a thread requests ahead
+constexpr int RL_BATCH = 2;          // 16-byte groups of logits a thread requests ahead (4 or 6: more code, slower)
 constexpr int RL_TOUCH = 2048;       // touched ids a CTA lists; where there are more it goes through its counts
 constexpr int RL_LIST = 512;         // bias entries of a CTA's ids that it keeps; a longer list is searched where it stands
 constexpr int RL_LOCAL = 16384;      // histories up to here are scanned by every CTA of the row
