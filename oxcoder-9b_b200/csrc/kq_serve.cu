@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <new>
 
 using namespace kq;
@@ -109,6 +110,62 @@ static int pages_check(const kq_page_desc* d) {
   return KQ_OK;
 }
 
+// Scratches of freed handles, kept for the next ones: a server makes and drops handles while it runs, and an
+// allocation and its release cost a millisecond and a synchronisation each. Between launches a scratch's
+// tickets are zero, so it can be handed on as it is.
+constexpr size_t SCRATCH_PART = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
+constexpr int SCRATCH_KEEP = 4;      // per device
+static std::mutex g_scratch_mu;
+static struct { AttendScratch s[SCRATCH_KEEP]; int n; } g_scratch[16];
+
+static cudaError_t scratch_take(int device, AttendScratch& out) {
+  {
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    auto& kept = g_scratch[device];
+    if (kept.n) {
+      out = kept.s[--kept.n];
+      return cudaSuccess;
+    }
+  }
+  void* p = nullptr;
+  cudaError_t e = cudaMalloc(&p, SCRATCH_PART + PA_MAX_CTAS * sizeof(int));
+  if (e != cudaSuccess) return e;
+  out.part = static_cast<float*>(p);
+  out.ticket = reinterpret_cast<int*>(static_cast<char*>(p) + SCRATCH_PART);
+  e = cudaMemset(out.ticket, 0, PA_MAX_CTAS * sizeof(int));
+  if (e == cudaSuccess) e = cudaStreamSynchronize(0);   // the first call may be on a stream that does not wait for this one
+  if (e != cudaSuccess) {
+    cudaFree(p);
+    out = AttendScratch{};
+  }
+  return e;
+}
+static void scratch_give(int device, const AttendScratch& s) {
+  if (cudaSetDevice(device) != cudaSuccess) return;
+  if (cudaDeviceSynchronize() == cudaSuccess) {         // no launch still uses it
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    auto& kept = g_scratch[device];
+    if (kept.n < SCRATCH_KEEP) {
+      kept.s[kept.n++] = s;
+      return;
+    }
+  }
+  cudaFree(s.part);
+}
+// The attention kernels' shared memory, allowed once per device (which is current).
+static cudaError_t attend_setup(int device, int type, int hd) {
+  static std::atomic<unsigned> done[16];
+  const int at = (type - KQ_F16) * 3 + (hd == 64 ? 0 : hd == 128 ? 1 : 2);
+  if (done[device].load(std::memory_order_acquire) >> at & 1u) return cudaSuccess;
+  for (int v = 0; v < 4; ++v) {
+    const AttendKernel k = attend_kernel(type, hd, v & 1, v & 2);
+    const cudaError_t e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+    if (e != cudaSuccess) return e;
+  }
+  done[device].fetch_or(1u << at, std::memory_order_release);
+  return cudaSuccess;
+}
+
 kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
   const kq_page_desc* given = static_cast<const kq_page_desc*>(desc);
   KqhDevice dev;
@@ -131,21 +188,12 @@ kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
   c->device = device;
   c->dev = dev;
   while ((1 << c->shift) < d->page) ++c->shift;
-  const size_t part = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
-  cudaError_t e = cudaSuccess;
-  if (with) {
+  cudaError_t e = attend_setup(device, d->type, d->head_dim);
+  if (e == cudaSuccess && with) {
     c->scratch = with->scratch;
     c->shared = true;
-  } else {
-    e = cudaMalloc(&c->scratch.part, part + PA_MAX_CTAS * sizeof(int));
-  }
-  if (e == cudaSuccess && !with) {
-    c->scratch.ticket = reinterpret_cast<int*>(reinterpret_cast<char*>(c->scratch.part) + part);
-    e = cudaMemset(c->scratch.ticket, 0, PA_MAX_CTAS * sizeof(int));
-  }
-  for (int v = 0; v < 4 && e == cudaSuccess; ++v) {
-    const AttendKernel k = attend_kernel(d->type, d->head_dim, v & 1, v & 2);
-    e = cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
+  } else if (e == cudaSuccess) {
+    e = scratch_take(device, c->scratch);
   }
   if (e != cudaSuccess) {
     kqh_error(e == cudaErrorMemoryAllocation ? KQ_ERR_MEMORY : KQ_ERR_BACKEND,
@@ -160,10 +208,7 @@ extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) { return
 
 extern "C" void kq_pages_free(kq_pages* c) {
   if (!c) return;
-  if (c->scratch.part && !c->shared) {
-    cudaSetDevice(c->device);
-    cudaFree(c->scratch.part);
-  }
+  if (c->scratch.part && !c->shared) scratch_give(c->device, c->scratch);
   delete c;
 }
 

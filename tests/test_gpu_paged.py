@@ -495,3 +495,30 @@ def test_both_ways_of_passing_tensors_agree(env, monkeypatch):
             got.append((k, v, qo, out, z, best))
         for a, b in zip(*got):
             assert torch.equal(a, b)
+
+
+def test_many_handles_and_streams(env):
+    """Handles that come and go, on streams of their own that do not wait for the default one."""
+    K, torch = env
+    g = torch.Generator(device="cuda").manual_seed(10)
+    k, v = make_pool(torch, g, 64, 2, 16, 128, "float16")
+    t = dict(dtype=torch.int32, device="cuda")
+    table, lens = torch.arange(64, **t).view(1, 64), torch.tensor([1000], **t)
+    q = torch.randn((1, 8, 128), device="cuda", generator=g)
+    want, err = attend_exact(f64(q), f64(k), f64(v), None, None, table.cpu().numpy(), [1000], 16, 0, 128 ** -0.5)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    for _ in range(3):
+        caches = [K.PagedCache(k, v) for _ in streams]
+        outs = [torch.empty_like(q) for _ in streams]
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for c, o, s in zip(caches, outs, streams):
+                c.attend(q, table, lens, o, stream=s.cuda_stream)
+        for s in streams:
+            K.check_stream(stream=s.cuda_stream)
+        for o in outs:
+            check_attend(f64(o), want, err, 0.0, "float32")
+            assert torch.equal(o, outs[0])
+        for c in caches:
+            c.close()

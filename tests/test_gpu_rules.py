@@ -192,3 +192,55 @@ def test_rules_refusals(env):
         K.logit_rules(z.double(), z.double())
     K.logit_rules(z[:0], z[:0].clone())
     K.check_stream()
+
+
+@pytest.mark.parametrize("kind,V,ld", [("bfloat16", 20011, 1), ("float16", 9001, 3), ("float32", 5003, 2), ("bfloat16", 40000, 0)])
+def test_equal_maxima_take_the_lowest_id(env, kind, V, ld):
+    """Ties between ids anywhere in a row: its ends, its touched ids, ids of other CTAs, masked ones."""
+    K, torch = env
+    rng = np.random.default_rng(V)
+    n = 24
+    z = torch.tensor(rng.normal(0, 1, (n, V + ld)).astype(np.float32), device="cuda").to(getattr(torch, kind))[:, :V]
+    want, hist, mask = [], np.full((n, 3), -1, np.int32), np.full((n, (V + 31) // 32), 0xffffffff, np.uint32)
+    for i in range(n):
+        ids = np.sort(rng.choice(V, 5, replace=False))
+        if i % 4 == 0:
+            ids[0] = i % 8
+        if i % 4 == 1:
+            ids[1:] = np.sort(V - 1 - rng.choice(20, 4, replace=False))
+        z[i, torch.tensor(ids, device="cuda")] = 16.0
+        hist[i, :2] = ids[:2] if i % 3 else ids[3:]     # touched, by rules that change nothing
+        if i % 5 == 4:                                  # the lowest is masked
+            mask[i, ids[0] // 32] &= ~np.uint32(1 << (ids[0] % 32))
+            ids = ids[1:]
+        want.append(int(ids[0]))
+    cu = lambda a: torch.tensor(a, device="cuda")  # noqa: E731
+    best = torch.zeros(n, dtype=torch.int32, device="cuda")
+    K.logit_rules(z, torch.empty((n, V + ld), dtype=z.dtype, device="cuda")[:, :V], best=best, hist=cu(hist),
+                  hist_len=torch.full((n,), 3, dtype=torch.int32, device="cuda"), repetition=torch.ones(n, device="cuda"),
+                  mask=cu(mask.view(np.int32)))
+    K.check_stream()
+    assert best.tolist() == want
+
+
+def test_long_histories_and_lists(env):
+    """Histories past 16-bit counts and past what every CTA scans, more touched ids and biases than a CTA lists."""
+    K, torch = env
+    rng = np.random.default_rng(5)
+    V, n, most, entries = 50021, 3, 40000, 3000
+    z = torch.tensor(rng.normal(0, 3, (n, V)).astype(np.float32), device="cuda")
+    hist = rng.integers(0, V, (n, most)).astype(np.int32)
+    hist[0, :] = 77                                     # 40000 times one id
+    hist_len = np.array([most, most, 16384], np.int32)
+    prompt = np.array([0, 20000, 100], np.int32)
+    ids = rng.integers(0, V, (n, entries)).astype(np.int32)
+    bias = rng.normal(0, 4, (n, entries)).astype(np.float32)
+    cu = lambda a: torch.tensor(a, device="cuda")  # noqa: E731
+    one = torch.ones(n, device="cuda")
+    out, best = torch.empty_like(z), torch.zeros(n, dtype=torch.int32, device="cuda")
+    K.logit_rules(z, out, best=best, hist=cu(hist), hist_len=cu(hist_len), prompt_len=cu(prompt), repetition=1.25 * one,
+                  frequency=0.5 * one, presence=0.25 * one, bias_ids=cu(ids), bias=cu(bias))
+    K.check_stream()
+    for i in range(n):
+        want, mag = exact(z[i].cpu().numpy(), hist[i, :hist_len[i]], int(prompt[i]), 1.25, 0.5, 0.25, ids[i], bias[i], None)
+        check_row(out[i].cpu().numpy().astype(np.float64), int(best[i]), want, mag, "float32")
