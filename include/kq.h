@@ -357,7 +357,7 @@ typedef struct {
   int n, vocab, type;                   /* KQ_F32, KQ_F16 or KQ_BF16 */
   int max_hist, n_bias, n_masks;
 } kq_rule_args;
-int kq_logit_rules(const kq_rule_args* a, int device, void* stream);
+int kq_logit_rules(const kq_rule_args* a, int device, void* stream);   /* the first call on a device sets it up: not in a capture */
 
 /* The same operators on tensor objects of a language binding, which would otherwise spend more time on
  * asking them for their addresses, shapes and strides than the kernels take. kq_tensor_source names the

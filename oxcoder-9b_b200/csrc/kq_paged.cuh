@@ -105,7 +105,8 @@ __device__ __forceinline__ void ap_store(void* p, const float (&x)[V]) {
 // Bound by memory: each source row is read and each stored row written once, in 16-byte loads. Grid
 // (token, slice of its head rows); a thread owns V pairs (j, j + rot / 2), V = 16 bytes of the source type, or 2 V
 // dims that do not turn, of U head rows: the rows' loads are all requested before the position is known,
-// and one look at the table and the angles serves them all.
+// and one look at the table and the angles serves them all. 8192 tokens of 32 + 2 x 8 bf16 heads of 128: 40.2 us, 5.1
+// TB/s, 0.78 of the copy rate (a row per thread 44.5); one token about 2.5 us, all of it latency.
 constexpr int AP_THREADS = 128;
 constexpr int AP_DEEP = 3;   // head rows per thread of a large append
 template <int ST, int CT, int U>
@@ -326,8 +327,9 @@ struct PaShape {
   static_assert(STAGES >= 2, "a ring of two slots at least");
   static constexpr int SMEM = PA_WARPS * STAGES * STAGE + QBYTES;
 };
-constexpr int PA_JOIN = 16;                    // partials of a chain read at once
-constexpr int PA_COST = 3;                     // what a (sequence, head) costs beside its tiles, in tiles
+constexpr int PA_JOIN = 16;                    // partials of a chain read at once (24, 32: more code, not faster)
+constexpr int PA_COST = 3;                     // what a (sequence, head) costs beside its tiles, in tiles (128 ragged
+                                               // sequences at 1 / 2 / 3 / 5: 90 / 72 / 68 / 71 us)
 constexpr int PA_PLD = 256 + 4;                // floats of a scratch row (the widest head_dim)
 
 struct AttendScratch {
@@ -347,9 +349,13 @@ struct PaCursor {
   KeyRange R;
 };
 
+// Bound by memory where runs are long: 64 sequences of 8K to 32K keys (fp16, 32/8 heads of 128) 785 to 828 us,
+// 6.0 to 6.3 TB/s of K/V, 0.91 to 0.96 of the copy rate; 128 sequences of 9 to 4096 keys 65 to 68 us (floor 49); by
+// latency where they are short: one sequence of 4096 keys 13.2 us (lengths, table, keys, two steps and the
+// join follow one another; a step costs about 1.1 us of a warp's dependent instructions).
 // The work is cut into equal runs of units, one per CTA, in the order sequence, head, 64-key tile,
-// wherever sequences end: CTAs finish together whatever the lengths are (cutting by tiles alone left the
-// CTAs with many short sequences 4 times behind the others). A CTA walks its run segment by segment
+// wherever sequences end: CTAs finish together whatever the lengths are (cut by tiles alone, the CTAs
+// with many short sequences were 4 times behind the others). A CTA walks its run segment by segment
 // (one sequence and head at a time). Each warp owns a ring of slots and fills it STAGES - 1 steps
 // ahead, across segment borders: a segment's query rows first, then its steps of 16 keys, so nothing
 // but the last slots of a run is waited for in full. A segment that is a whole (sequence, head) is

@@ -88,16 +88,20 @@ template <> struct RlCount<true> { using type = uint32_t; static constexpr uint3
 
 // Bound by memory: a row is read and written once. A small cluster of CTAs owns a row, its ids dealt out
 // in turns of RL_THREADS 16-byte groups (the frequent ids of a vocabulary lie together: consecutive
-// shares gave one CTA of each row most of the touched ids). First the CTA counts its ids' occurrences in shared memory: a short history is
-// scanned by every CTA of the row (16 KB from the L2 each, no barrier between CTAs), a long one (over
-// RL_LOCAL) by its parts, with the hits sent to the owner's shared memory. The first to count an id
-// lists it. Then the CTA's logits stream through registers, RL_BATCH groups of 16 bytes a thread ahead (the
-// first batch flies during the scan): mask, write, pick among the untouched; and last the listed ids, a
-// thread each. (Touched ids handled within the stream cost every warp their whole latency at almost every
-// step: 128 rows with up to 4096 tokens took 124 us.) Counts are integer adds and the last bias entry is
-// a maximum, so nothing depends on the order of arrival.
+// shares gave one CTA of each row most of the touched ids). First the CTA counts its ids' occurrences
+// in shared memory: a short history is scanned by every CTA of the row (16 KB from the L2 each, no
+// barrier between CTAs), a long one (over RL_LOCAL) by its parts, with the hits sent to the owner's
+// shared memory. The first to count an id lists it. Then the CTA's logits stream through registers,
+// RL_BATCH groups of 16 bytes a thread ahead (the first batch flies during the scan): mask, write, pick
+// among the untouched; and last the listed ids, a thread each. (Touched ids handled within the stream
+// cost every warp their whole latency at almost every step.) Counts are integer adds and the last
+// bias entry is a maximum, so nothing depends on the order of arrival.
 // Positions count from the 16-byte boundary at or below the row's start (u = id + shift), so rows of
 // any alignment move in 16-byte groups; only the groups over a row's ends are handled element by element.
+// Measured: 128 fp32 rows of 151936 with histories of up to 4096 tokens, 300 biases and masks 48.9 us (3.2
+// TB/s read and written; the copy rate would take 23.8: two waves of CTAs, each counting before it
+// streams); in the stream 124, one CTA per row 240, clusters of 16 with the logits held meanwhile 109
+// to 119 (a cluster waits until 16 slots of one GPC are free). One row 6.9 us.
 template <typename T, bool LONG>
 __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_constant__ RuleParams P) {
   using Count = typename RlCount<LONG>::type;

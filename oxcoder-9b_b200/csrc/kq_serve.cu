@@ -217,7 +217,7 @@ static PageTable table_of(const kq_pages* c, const int32_t* table, const int32_t
 }
 static bool table_ok(const kq_pages* c, const int32_t* table, const int32_t* seq, long long ld, int n_seq, int max_pages, int n) {
   return table && n_seq >= 1 && max_pages >= 1 && ld >= max_pages && (seq || n <= n_seq) &&
-         (long long)max_pages * c->d.page <= 0x7fffffffll;
+         (long long)max_pages * c->d.page <= 0x7ffff000ll;   // keys and the tiles over a sequence's end are 32-bit
 }
 
 extern "C" int kq_page_append(kq_pages* c, const kq_append_args* given, void* stream) {

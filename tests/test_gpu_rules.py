@@ -74,6 +74,7 @@ def check_row(got, best, want, mag, kind):
     ("float16", 6, 5001, 400, 7, 2, 3, True),
     ("bfloat16", 3, 393216, 2000, 50, 3, 0, False),
     ("float16", 2, 65537, 0, 0, 2, 0, False),
+    ("float32", 1, 393216, 20000, 10, 1, 0, False),
 ])
 def test_rules(env, kind, n, V, most, entries, masks, ld, inplace):
     K, torch = env
@@ -244,3 +245,23 @@ def test_long_histories_and_lists(env):
     for i in range(n):
         want, mag = exact(z[i].cpu().numpy(), hist[i, :hist_len[i]], int(prompt[i]), 1.25, 0.5, 0.25, ids[i], bias[i], None)
         check_row(out[i].cpu().numpy().astype(np.float64), int(best[i]), want, mag, "float32")
+
+
+def test_captured_and_on_a_stream_of_its_own(env):
+    K, torch = env
+    z = torch.randn((3, 70001), device="cuda")
+    out, best = torch.empty_like(z), torch.zeros(3, dtype=torch.int32, device="cuda")
+    ids = torch.tensor([[5], [70000], [-1]], dtype=torch.int32, device="cuda")
+    bias = torch.full((3, 1), 50.0, device="cuda")
+    K.logit_rules(z, out, best=best, bias_ids=ids, bias=bias)
+    s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        K.logit_rules(z, out, best=best, bias_ids=ids, bias=bias, stream=s.cuda_stream)
+        K.logit_rules(out, out, best=best, bias_ids=ids, bias=bias, stream=s.cuda_stream)
+    z.normal_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert best.tolist() == [5, 70000, int(z[2].argmax())]
+    assert float(out[0, 5]) == float(z[0, 5] + 50.0 + 50.0) and torch.equal(out[2], z[2])
+    K.check_stream()
