@@ -153,7 +153,9 @@ __global__ void __launch_bounds__(AP_THREADS) k_page_append(const __grid_constan
   }
   if (page < 0 || page >= P.T.n_pages) {
     if (r0 + (U - 1) * rstep >= P.n_heads)
-      atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW : pi >= P.T.max_pages ? KQ_DEV_ERR_BAD_POS : KQ_DEV_ERR_BAD_PAGE);
+      atomicOr(P.err, s < 0 || s >= P.T.n_seq ? KQ_DEV_ERR_BAD_ROW
+                      : pi >= P.T.max_pages   ? KQ_DEV_ERR_BAD_POS
+                                              : KQ_DEV_ERR_BAD_PAGE);
     page = -1;
   }
   const int row = pos & ((1 << P.T.page_shift) - 1);
@@ -362,7 +364,8 @@ struct PaCursor {
 // written out; otherwise its (o, m, l) goes to the scratch and the last CTA of the chain to arrive
 // joins the chain's partials in CTA order, so the sums' order is fixed.
 template <int CT, int HD, int NT, bool PREC>
-__global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_SM) k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
+__global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_SM)
+k_page_attend(const __grid_constant__ AttendParams P, const AttendScratch W) {
   using S = PaShape<CT, HD, NT, PREC>;
   constexpr bool BF = S::BF, E8 = CT == PG_E4M3;
   constexpr int KS = S::KS, NQ = S::NQ, NP = S::NP;
@@ -431,7 +434,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
   // rows without a key: zeros
   for (int i = blockIdx.x; i < P.n; i += gridDim.x) {
     if (units_of(i)) continue;
-    for (int e = tid; e < P.n_heads * HD; e += PA_WARPS * 32) pg_store(P.out, P.type, i * P.o_tok + (e / HD) * P.o_head + e % HD, 0.f);
+    for (int e = tid; e < P.n_heads * HD; e += PA_WARPS * 32)
+      pg_store(P.out, P.type, i * P.o_tok + (e / HD) * P.o_head + e % HD, 0.f);
   }
   __syncthreads();
   if (begin >= end) return;
@@ -643,7 +647,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
           pa_ldsm(kb + ks * 16, r);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t a[4] = {pa_e4m3x2(r[2 * j]), pa_e4m3x2(r[2 * j + 1]), pa_e4m3x2(r[2 * j] >> 16), pa_e4m3x2(r[2 * j + 1] >> 16)};
+            const uint32_t a[4] = {pa_e4m3x2(r[2 * j]), pa_e4m3x2(r[2 * j + 1]), pa_e4m3x2(r[2 * j] >> 16),
+                                   pa_e4m3x2(r[2 * j + 1] >> 16)};
             score(ks + j, a);
           }
         }
@@ -668,7 +673,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
           // an infinite key makes the leading term's sum infinite and a zero lower term's sum NaN
           float a = s[NQ - 1][nt][e];
 #pragma unroll
-          for (int j = NQ - 2; j >= 0; --j) a = j > 0 || fabsf(s[0][nt][e]) < INFINITY ? __fadd_rn(a, s[j][nt][e]) : s[0][nt][e];
+          for (int j = NQ - 2; j >= 0; --j)
+            a = j > 0 || fabsf(s[0][nt][e]) < INFINITY ? __fadd_rn(a, s[j][nt][e]) : s[0][nt][e];
           x[e] = (e < 2 ? va : vb8) ? __fmul_rn(a, sc[nt][e & 1]) : -INFINITY;
         }
 #pragma unroll
@@ -771,8 +777,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, PaShape<CT, HD, NT, PREC>::PER_
         L = __fmaf_rn(wt, row[HD + 1], L);
         O = __fmaf_rn(wt, row[d], O);
       }
-      if (whole) pg_store(P.out, P.type, cur.seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
-      else {
+      if (whole) {
+        pg_store(P.out, P.type, cur.seq * P.o_tok + (h0 + h) * P.o_head + d, L == 0.f ? 0.f : __fdiv_rn(O, L) * vscale);
+      } else {
         __stcg(part + h * PA_PLD + d, O);
         if (d == 0) {
           __stcg(part + h * PA_PLD + HD, M);

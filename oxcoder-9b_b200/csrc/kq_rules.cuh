@@ -83,8 +83,16 @@ constexpr int RL_LOCAL = 16384;      // histories up to here are scanned by ever
 
 // Counts of a CTA's ids in shared memory: 16 bits an id, or 32 where histories may be longer. Beside the
 // count: the id is in the prompt, has a bias.
-template <bool LONG> struct RlCount { using type = uint16_t; static constexpr uint32_t PROMPT = 0x8000u, BIASED = 0x4000u, MOST = 0x3fffu; };
-template <> struct RlCount<true> { using type = uint32_t; static constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, MOST = 0x3fffffffu; };
+template <bool LONG>
+struct RlCount {
+  using type = uint16_t;
+  static constexpr uint32_t PROMPT = 0x8000u, BIASED = 0x4000u, MOST = 0x3fffu;
+};
+template <>
+struct RlCount<true> {
+  using type = uint32_t;
+  static constexpr uint32_t PROMPT = 0x80000000u, BIASED = 0x40000000u, MOST = 0x3fffffffu;
+};
 
 // Bound by memory: a row is read and written once. A small cluster of CTAs owns a row, its ids dealt out
 // in turns of RL_THREADS 16-byte groups (the frequent ids of a vocabulary lie together: consecutive
@@ -138,7 +146,8 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   // turns [t_lo, t_hi) lie inside the row, both rows aligned alike: whole groups, no checks
   const int turns = u_end > rank * STEP ? (u_end - rank * STEP - 1) / (ranks * STEP) + 1 : 0;
   const int t_lo = rank == 0 && shift ? 1 : 0;
-  const int t_hi = vec_out ? max(t_lo, (u_end - rank * STEP) / STEP > 0 ? ((u_end - rank * STEP) / STEP - 1) / ranks + 1 : 0) : t_lo;
+  const int inside = (u_end - rank * STEP) / STEP;                       // whole turns of the row from this CTA's first on
+  const int t_hi = vec_out && inside > 0 ? max(t_lo, (inside - 1) / ranks + 1) : t_lo;
   const int first = tid * VEC - shift;                                   // id of this thread's group in the turn at 0
   uint4 x[RL_BATCH];
   auto request = [&](int turn) {

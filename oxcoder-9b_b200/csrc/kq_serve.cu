@@ -259,7 +259,8 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* given, void* st
   const int slices = (rows * units + AP_THREADS - 1) / AP_THREADS;
   const bool deep = (long long)a->n * slices > 64ll * c->dev.nsm;
   const dim3 grid((unsigned)a->n, (unsigned)(deep ? (slices + AP_DEEP - 1) / AP_DEEP : slices));
-  CU(launch(deep ? append_kernel<AP_DEEP>(a->src_type, c->d.type) : append_kernel<1>(a->src_type, c->d.type), grid, AP_THREADS, 0, stream, 1, P));
+  const AppendFn fn = deep ? append_kernel<AP_DEEP>(a->src_type, c->d.type) : append_kernel<1>(a->src_type, c->d.type);
+  CU(launch(fn, grid, AP_THREADS, 0, stream, 1, P));
   return KQ_OK;
 }
 
@@ -303,8 +304,9 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* st
 
 typedef void (*RulesFn)(RuleParams);
 static RulesFn rules_kernel(int type, bool deep) {
-  if (deep) return type == KQ_F32 ? k_logit_rules<float, true> : type == KQ_F16 ? k_logit_rules<__half, true> : k_logit_rules<__nv_bfloat16, true>;
-  return type == KQ_F32 ? k_logit_rules<float, false> : type == KQ_F16 ? k_logit_rules<__half, false> : k_logit_rules<__nv_bfloat16, false>;
+  if (type == KQ_F32) return deep ? k_logit_rules<float, true> : k_logit_rules<float, false>;
+  if (type == KQ_F16) return deep ? k_logit_rules<__half, true> : k_logit_rules<__half, false>;
+  return deep ? k_logit_rules<__nv_bfloat16, true> : k_logit_rules<__nv_bfloat16, false>;
 }
 // Shared memory and cluster sizes above the defaults, allowed once per device (which is current).
 static int rules_setup(int device) {

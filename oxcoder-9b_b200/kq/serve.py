@@ -173,8 +173,9 @@ class PagedCache(object):
         if not self.h:
             raise ValueError("the cache is closed")
         T = _Direct.type
-        if type(k) is T and type(v) is T and type(table) is T and type(pos) is T and (rope is None or (type(rope[0]) is T and type(rope[1]) is T)) \
-                and (seq is None or type(seq) is T) and (q is None or (type(q) is T and type(q_out) is T)):
+        if type(k) is T and type(v) is T and type(table) is T and type(pos) is T and (seq is None or type(seq) is T) \
+                and (rope is None or (type(rope[0]) is T and type(rope[1]) is T)) \
+                and (q is None or (type(q) is T and type(q_out) is T)):
             rc = _Direct.page_append(self.h, id(k), id(v), id(table), id(pos), None if seq is None else id(seq),
                                      None if rope is None else id(rope[0]), None if rope is None else id(rope[1]),
                                      None if q is None else id(q), None if q_out is None else id(q_out), stream)
