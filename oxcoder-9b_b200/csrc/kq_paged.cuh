@@ -351,8 +351,8 @@ struct PaCursor {
   KeyRange R;
 };
 
-// Bound by memory where runs are long: 64 sequences of 8K to 32K keys (fp16, 32/8 heads of 128) 785 to 828 us,
-// 6.0 to 6.3 TB/s of K/V, 0.91 to 0.96 of the copy rate; 128 sequences of 9 to 4096 keys 65 to 68 us (floor 49); by
+// Bound by memory where runs are long: 64 sequences of 8K to 32K keys (fp16, 32/8 heads of 128) 785 to 839 us,
+// 5.9 to 6.3 TB/s of K/V, 0.90 to 0.96 of the copy rate; 128 sequences of 9 to 4096 keys 65 to 69 us (floor 49); by
 // latency where they are short: one sequence of 4096 keys 13.2 us (lengths, table, keys, two steps and the
 // join follow one another; a step costs about 1.1 us of a warp's dependent instructions).
 // The work is cut into equal runs of units, one per CTA, in the order sequence, head, 64-key tile,
