@@ -482,7 +482,7 @@ extern "C" int kq_logit_rules_tensors(void* logits, void* out, void* best, void*
   if (bias)
     FITS(tensor_of(bias_id, 2, ti) && ti.type == T_I32 && ti.device == dev && ti.n[0] == n && tensor_of(bias, 2, tv) &&
          tv.type == KQ_F32 && tv.device == dev && tv.n[0] == n && tv.n[1] == ti.n[1] && (n == 1 || tv.s[0] == ti.s[0]));
-  if (mask) FITS(tensor_of(mask, 2, tm) && tm.type == T_I32 && tm.device == dev);
+  if (mask) FITS(tensor_of(mask, 2, tm) && tm.type == T_I32 && tm.device == dev && tm.n[1] >= (tl.n[1] + 31) / 32);
   if (mask_row) FITS(vector_as(mask_row, T_I32, dev, n, tmr));
   kq_rule_args a{};
   auto ld = [](const Tensor& t) { return t.n[0] > 1 ? t.s[0] : t.n[1]; };
