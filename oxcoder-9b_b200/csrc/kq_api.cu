@@ -1000,7 +1000,7 @@ static kq_model* model_create(const kq_config* cfg, int device, int rank, int wo
     m->hticket = dalloc<int>(m, 1, ok);
     m->st = dalloc<DecodeState>(m, 1, ok);
     m->out_cap = c.ctx;
-    m->out_ids = dalloc<int>(m, (size_t)m->out_cap, ok);
+    m->out_ids = dalloc<int>(m, (size_t)std::max(m->out_cap, (int)MM_MAXM), ok);   // a batched step's rows may outnumber the context
     m->err = dalloc<int>(m, 1, ok);
     if (cudaMallocHost(&m->st_host, sizeof(DecodeState)) != cudaSuccess) ok = false;
   }
