@@ -54,6 +54,10 @@ __device__ __forceinline__ uint32_t rl_ranks() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// The cluster's first barrier phase, in two halves: arrived at as the kernel starts, waited for before the first
+// access to another CTA's shared memory, which may be touched only once that CTA runs.
+__device__ __forceinline__ void rl_started() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void rl_all_started() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ void rl_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -118,6 +122,7 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   extern __shared__ __align__(16) uint8_t rl_smem[];
   __shared__ float s_v[RL_THREADS / 32], s_cv[RL_CLUSTER], s_bias[RL_LIST];
   __shared__ int s_i[RL_THREADS / 32], s_ci[RL_CLUSTER], s_entry[RL_LIST], s_id[RL_LIST], s_touched[RL_TOUCH], s_entries, s_n;
+  rl_started();
   const int tid = threadIdx.x, rank = (int)rl_rank(), ranks = (int)rl_ranks(), i = blockIdx.x / ranks, span = P.span;
   Count* cnt = reinterpret_cast<Count*>(rl_smem);                                    // [span]
   const bool counted = P.hist || P.n_bias;
@@ -184,8 +189,12 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
   auto mask_of = [&](int id) { return mask ? mask[id >> 5] : 0xffffffffu; };
   const bool apart = nh > RL_LOCAL;                       // the same for all CTAs of the row
   if (counted) {
-    if (apart) rl_cluster_sync();                         // every CTA's counts are zero
-    else __syncthreads();
+    if (apart) {
+      rl_all_started();
+      rl_cluster_sync();                                  // every CTA's counts are zero
+    } else {
+      __syncthreads();
+    }
     // adds to, or sets bits of, the count of one of this CTA's ids (h < 0: none), and lists it if it was 0; whole warps
   auto mark = [&](int h, uint32_t v, bool bits) {
       bool first = false;
@@ -367,6 +376,7 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
       }
     }
   }
+  if (!(counted && apart)) rl_all_started();
   if (!P.best) return;
   // ---- the greedy id: warp, CTA, cluster
 #pragma unroll

@@ -38,3 +38,21 @@ def test_narrow_masks_are_refused(env, way):
         with pytest.raises(ValueError, match="too few words"):
             K.logit_rules(z, out, mask=mask, mask_row=torch.zeros(2, dtype=torch.int32, device="cuda"))
     K.check_stream()
+
+
+@pytest.mark.parametrize("vocab,kind", [(4097, "float32"), (6145, "float32"), (16390, "float32"), (8200, "bfloat16"), (40, "float16")])
+def test_clusters_whose_last_blocks_have_little_to_do(env, vocab, kind):
+    """Rows cut so that some blocks of a cluster own no id, or one group: they are done before the others begin."""
+    K, torch = env
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    ids = torch.empty((60, 2), dtype=torch.int32, device="cuda")
+    want = torch.empty_like(ids)
+    for n in (1, 2):
+        z = torch.randn((60, n, vocab), device="cuda", generator=g).to(getattr(torch, kind))
+        out = torch.empty_like(z)
+        for i in range(60):
+            K.logit_rules(z[i], out[i], best=ids[i, :n])
+        top = z.float().amax(2, keepdim=True)
+        want[:, :n] = torch.where(z.float() == top, torch.arange(vocab, device="cuda", dtype=torch.int32), vocab).amin(2)
+        K.check_stream()
+        assert torch.equal(ids[:, :n], want[:, :n]) and torch.equal(out, z)
