@@ -56,8 +56,8 @@ __device__ __forceinline__ uint32_t rl_ranks() {
 }
 // The cluster's first barrier phase, in two halves: arrived at as the kernel starts, waited for before the first
 // access to another CTA's shared memory, which may be touched only once that CTA runs.
-__device__ __forceinline__ void rl_started() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void rl_all_started() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void rl_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;"); }
+__device__ __forceinline__ void rl_all_started() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void rl_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
     if (apart) rl_cluster_sync();                         // every hit has arrived
     else __syncthreads();
   }
+  if (!(counted && apart)) rl_all_started();              // by now they do (waited for after the stream: 45 16-bit rows 10.8 us, here 10.4)
 
   // ---- the stream: masks and writes every id, picks among the untouched. It keeps its largest value and
   // that value's turn; the id is looked up once, at the end.
@@ -376,7 +377,6 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
       }
     }
   }
-  if (!(counted && apart)) rl_all_started();
   if (!P.best) return;
   // ---- the greedy id: warp, CTA, cluster
 #pragma unroll
