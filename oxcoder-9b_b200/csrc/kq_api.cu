@@ -75,6 +75,13 @@ static GmFn gm_fn(int nw, int nb, int C, int ty) {
   return nb == 2 ? gm_fn_for<12, 2, 2>(C) : gm_fn_for<12, 1, 2>(C);
 }
 
+// Zeroes device memory and waits until it is zero. A cudaMemset alone returns at once and runs on the legacy stream,
+// which the streams of models, and of callers, need not wait for: it could erase what they store meanwhile.
+static cudaError_t zero_now(void* p, size_t bytes) {
+  const cudaError_t e = cudaMemset(p, 0, bytes);
+  return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
+}
+
 // ------------------------------------------------------------------------------ per-device context
 struct DevCtx {
   bool init = false;
@@ -131,7 +138,7 @@ static int dev_init(int device) {
     d.tmv_smem = (ev && std::atoi(ev) == 1) ? budget : 0;
   }
   CU(cudaMalloc(&d.err, 2 * sizeof(int)));   // [0] matrix-hook calls, [1] serving operators (kq_serve.cu)
-  CU(cudaMemset(d.err, 0, 2 * sizeof(int)));
+  CU(zero_now(d.err, 2 * sizeof(int)));
   d.init = true;
   return KQ_OK;
 }
@@ -888,8 +895,8 @@ template <typename T>
 static T* dalloc(kq_model* m, size_t n, bool& ok) {
   void* p = nullptr;
   if (cudaMalloc(&p, n * sizeof(T)) != cudaSuccess) { ok = false; return nullptr; }
-  cudaMemset(p, 0, n * sizeof(T));
   m->allocs.push_back(p);
+  if (zero_now(p, n * sizeof(T)) != cudaSuccess) { ok = false; return nullptr; }
   return reinterpret_cast<T*>(p);
 }
 
@@ -2702,7 +2709,7 @@ static int qmat_gemv_params(kq_qmat* a, const float* x_dev, float* y_dev, Matvec
   if (D.tmv_smem > 0 && !a->tv_part) {
     if (cudaMalloc(&a->tv_part, (size_t)D.nsm * 2 * TV_ROWS * 4) != cudaSuccess ||
         cudaMalloc(&a->tv_ticket, (size_t)TV_MAX_TILES * 4) != cudaSuccess ||
-        cudaMemset(a->tv_ticket, 0, (size_t)TV_MAX_TILES * 4) != cudaSuccess)
+        zero_now(a->tv_ticket, (size_t)TV_MAX_TILES * 4) != cudaSuccess)
       return set_err(KQ_ERR_MEMORY, "matvec scratch");
   }
   L.tmv = !L.pl.mma && tmv_plan(L.p, D.nsm, D.tmv_smem, a->tv_part, a->tv_ticket, L.t, L.grid);

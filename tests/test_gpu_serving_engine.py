@@ -35,3 +35,38 @@ def test_more_sequences_than_positions(env):
         got.append((ids, one))                           # the two paths round differently: each against itself
         e.close()
     assert got[0] == got[1]
+
+
+@pytest.mark.parametrize("kind", ["paged", "batch"])
+def test_caches_made_on_a_used_engine_while_the_default_stream_is_busy(env, kind):
+    """The zeroing of a new pool is over when the call returns: it cannot erase what the first step stores."""
+    K, torch = env
+    prompt = [int(v) for v in np.random.default_rng(6).integers(0, CFG["vocab"], 120)]
+
+    def ids(busy):
+        e = engine(K, n_layers=1)
+        e.feed_batch(prompt[:64], 0)                     # the batched pass's buffers are there
+        if busy:
+            x = torch.randn((4096, 4096), device="cuda")
+            for _ in range(200):                         # some tens of milliseconds
+                x = (x @ x).clamp_(-1, 1)
+        if kind == "paged":
+            e.paged_caches(600, 1024, max_seq=1)
+            table = np.array([[599]])
+            e.paged_step(table, [0] * 119, prompt[:119], range(119), pick=False)
+            got, t = [], prompt[119]
+            for i in range(6):
+                t = e.paged_step(table, [0], [t], [119 + i])[0]
+                got.append(t)
+        else:
+            e.batch_caches(300)
+            e.batch_feed(299, prompt[:119], 0)
+            got, t = [], prompt[119]
+            for i in range(6):
+                t = e.batch_step([299], [t], [119 + i])[0]
+                got.append(t)
+        torch.cuda.synchronize()
+        e.close()
+        return got
+
+    assert ids(True) == ids(False)
