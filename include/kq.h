@@ -190,7 +190,8 @@ int kq_batch_step(kq_model* m, const int32_t* seqs, const int32_t* toks, const i
  * (consecutive positions of one) or both at once; (sequence, position) pairs must be distinct. out null:
  * the tokens are only fed. Otherwise out[i] gets row i's greedy id under the rules: null (none), or
  * kq_logit_rules' arguments for n rows (device tensors, ready on `stream`; logits, out, best, n, vocab
- * and type are the step's own), -1 where a row's rules allow nothing. */
+ * and type are the step's own), -1 where a row's rules allow nothing. A step reports what its own kernels flagged
+ * (a mask row out of range: KQ_ERR_ARG, the ids are written), never another caller's flags. */
 int kq_paged_caches(kq_model* m, int n_pages, int page, int max_seq);
 
 /* ------------------------------------------------------------------ matrix hooks
@@ -377,7 +378,8 @@ int kq_logit_rules_tensors(void* logits, void* out, void* best, void* hist, void
 int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int max_pages, const int32_t* seqs, const int32_t* toks,
                   const int32_t* pos, int n, const kq_rule_args* rules, void* stream, int32_t* out);
 
-/* Waits for `stream` and reports (and clears) what the operators' kernels flagged on this device. */
+/* Waits for `stream` and reports (and clears, in one step) what the operators' kernels flagged on this device since the last
+ * check, whichever stream they ran on; a model's own steps (kq_paged_step) report their flags themselves. */
 int kq_stream_check(int device, void* stream);
 
 /* ------------------------------------------------------------------ prompt-lookup drafter

@@ -137,8 +137,8 @@ static int dev_init(int device) {
     const char* ev = std::getenv("KQ_TMV");   // opt-in while it is validated: 1 = the tensor-core GEMV
     d.tmv_smem = (ev && std::atoi(ev) == 1) ? budget : 0;
   }
-  CU(cudaMalloc(&d.err, 2 * sizeof(int)));   // [0] matrix-hook calls, [1] serving operators (kq_serve.cu)
-  CU(zero_now(d.err, 2 * sizeof(int)));
+  CU(cudaMalloc(&d.err, 3 * sizeof(int)));   // [0] matrix-hook calls, [1], [2] serving operators (kq_serve.cu)
+  CU(zero_now(d.err, 3 * sizeof(int)));
   d.init = true;
   return KQ_OK;
 }
@@ -1661,9 +1661,10 @@ static int check_dev_err(kq_model* m) {
   int e = 0;
   CU(cudaMemcpy(&e, m->err, sizeof(int), cudaMemcpyDeviceToHost));
   if (e) {
-    cudaMemset(m->err, 0, sizeof(int));
-    if (m->dec_bar) cudaMemset(m->dec_bar, 0, (size_t)(m->nph_all + 1) * sizeof(int));   // re-arm the phase counters
+    cudaMemsetAsync(m->err, 0, sizeof(int), m->stream);   // before the next call's kernels
+    if (m->dec_bar) cudaMemsetAsync(m->dec_bar, 0, (size_t)(m->nph_all + 1) * sizeof(int), m->stream);   // re-arm the phase counters
     if (e & (KQ_DEV_ERR_BAD_TOKEN | KQ_DEV_ERR_BAD_POS)) return set_err(KQ_ERR_ARG, "device saw an invalid token or position");
+    if (!(e & ~KQ_DEV_ERR_OPERANDS)) return set_err(KQ_ERR_ARG, "the step met device operands out of range:" + kqh_operands(e));
     char buf[96];
     std::snprintf(buf, sizeof buf, "a bounded device wait gave up (error bits 0x%x)", e);
     return set_err(KQ_ERR_TIMEOUT, buf);
@@ -2491,7 +2492,7 @@ extern "C" int kq_paged_caches(kq_model* m, int n_pages, int page, int max_seq) 
     d.k_head = d.v_head = (long long)page * c.head_dim;
     d.k_row = d.v_row = c.head_dim;
     d.type = KQ_F16; d.n_pages = n_pages; d.page = page; d.n_kv_heads = m->nkv_l; d.head_dim = c.head_dim;
-    kq_pages* p = kqh_pages_create(&d, m->device, l ? m->pages[0] : nullptr);
+    kq_pages* p = kqh_pages_create(&d, m->device, l ? m->pages[0] : nullptr, m->err);
     if (p) m->pages.push_back(p);
     else ok = false;
   }
@@ -2601,14 +2602,13 @@ extern "C" int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int m
     }
     R.logits = m->vlogits; R.out = m->vlogits; R.in_ld = R.out_ld = c.vocab; R.best = m->out_ids;
     R.n = M; R.vocab = c.vocab; R.type = KQ_F32;
-    if ((rc = kq_logit_rules(&R, m->device, s))) return rc;
+    if ((rc = kqh_logit_rules(&R, m->device, m->err, s))) return rc;
   }
   prof_mark(m, PC_END);
   if ((rc = tp_sync(m))) return rc;
   prof_flush(m);
   if (out) CU(cudaMemcpy(out, m->out_ids, M * sizeof(int32_t), cudaMemcpyDeviceToHost));
-  if ((rc = check_dev_err(m))) return rc;
-  return kq_stream_check(m->device, s);
+  return check_dev_err(m);
 }
 
 extern "C" int kq_commit(kq_model* m, const int32_t* path, int k, int pos) {

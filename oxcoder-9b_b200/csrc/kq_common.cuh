@@ -21,6 +21,7 @@ enum : int {
   KQ_DEV_ERR_BAD_PAGE = 64,     // a page id outside [0, n_pages) in a page table
   KQ_DEV_ERR_BAD_LEN = 128,     // a length past its table or array
   KQ_DEV_ERR_BAD_ROW = 256,     // a row index (page table, mask) out of range
+  KQ_DEV_ERR_OPERANDS = 8 | 16 | 64 | 128 | 256,   // the bits that name a bad operand (the others: a wait that gave up)
 };
 
 // Polls of mbarrier.try_wait before giving up. Each poll may suspend the thread for a

@@ -166,7 +166,7 @@ static cudaError_t attend_setup(int device, int type, int hd) {
   return cudaSuccess;
 }
 
-kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
+kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with, int* err) {
   const kq_page_desc* given = static_cast<const kq_page_desc*>(desc);
   KqhDevice dev;
   kq_page_desc own{}, *d = nullptr;
@@ -187,6 +187,7 @@ kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
   c->d = *d;
   c->device = device;
   c->dev = dev;
+  if (err) c->dev.err = err;
   while ((1 << c->shift) < d->page) ++c->shift;
   cudaError_t e = attend_setup(device, d->type, d->head_dim);
   if (e == cudaSuccess && with) {
@@ -204,7 +205,7 @@ kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with) {
   return c;
 }
 
-extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) { return kqh_pages_create(d, device, nullptr); }
+extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) { return kqh_pages_create(d, device, nullptr, nullptr); }
 
 extern "C" void kq_pages_free(kq_pages* c) {
   if (!c) return;
@@ -322,7 +323,8 @@ static int rules_setup(int device) {
   return KQ_OK;
 }
 
-extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
+int kqh_logit_rules(const void* args, int device, int* err, void* stream) {
+  const kq_rule_args* a = static_cast<const kq_rule_args*>(args);
   REQUIRE(a, "kq_logit_rules: null argument");
   REQUIRE(a->n >= 0 && a->vocab >= 1 && a->vocab <= KQ_RULES_MAX_VOCAB && a->n <= (1 << 26), "kq_logit_rules: bad row count or vocabulary size");
   REQUIRE(a->type == KQ_F32 || a->type == KQ_F16 || a->type == KQ_BF16, "kq_logit_rules: logits are f32, f16 or bf16");
@@ -344,7 +346,8 @@ extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   P.rep = a->repetition; P.freq = a->frequency; P.pres = a->presence;
   P.bias_id = a->bias_id; P.bias = a->bias; P.bias_ld = a->bias_ld;
   P.mask = a->mask; P.mask_row = a->mask_row; P.mask_ld = a->mask_ld;
-  P.n = a->n; P.vocab = a->vocab; P.max_hist = a->max_hist; P.n_bias = a->n_bias; P.n_masks = a->n_masks; P.err = dev.err;
+  P.n = a->n; P.vocab = a->vocab; P.max_hist = a->max_hist; P.n_bias = a->n_bias; P.n_masks = a->n_masks;
+  P.err = err ? err : dev.err;
   // 32-bit counts only where a history may hold more of one id than 14 bits count. The smallest
   // cluster whose CTAs hold at most RL_BYTES, then larger ones while the device has CTAs to spare.
   const bool deep = a->max_hist > (int)RlCount<false>::MOST;
@@ -359,6 +362,8 @@ extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) {
   CU(launch(rules_kernel(a->type, deep), dim3((unsigned)a->n * (unsigned)cl), RL_THREADS, (size_t)P.span * bytes, stream, cl, P));
   return KQ_OK;
 }
+
+extern "C" int kq_logit_rules(const kq_rule_args* a, int device, void* stream) { return kqh_logit_rules(a, device, nullptr, stream); }
 
 // ------------------------------------------------------------------------------ tensor objects
 // DLPack's DLTensor (its version 1 ABI).
@@ -498,19 +503,33 @@ extern "C" int kq_logit_rules_tensors(void* logits, void* out, void* best, void*
   return kq_logit_rules(&a, dev, stream);
 }
 
-extern "C" int kq_stream_check(int device, void* stream) {
-  KqhDevice dev;
-  const int rc = kqh_device(device, &dev);
-  if (rc) return rc;
-  CU(cudaStreamSynchronize((cudaStream_t)stream));
-  int e = 0;
-  CU(cudaMemcpy(&e, dev.err, sizeof(int), cudaMemcpyDeviceToHost));
-  if (!e) return KQ_OK;
-  CU(cudaMemset(dev.err, 0, sizeof(int)));
-  std::string what = "an operator met device operands out of range:";
+std::string kqh_operands(int e) {
+  std::string what;
+  if (e & KQ_DEV_ERR_BAD_TOKEN) what += " token";
   if (e & KQ_DEV_ERR_BAD_POS) what += " position";
   if (e & KQ_DEV_ERR_BAD_PAGE) what += " page id";
   if (e & KQ_DEV_ERR_BAD_LEN) what += " length";
   if (e & KQ_DEV_ERR_BAD_ROW) what += " row index";
-  return kqh_error(KQ_ERR_ARG, what);
+  return what;
+}
+
+// Reads and clears an error word in one step: what another stream's kernel flags meanwhile is kept for the next check.
+__global__ void k_take_flags(int* word, int* taken) { *taken = atomicExch(word, 0); }
+
+extern "C" int kq_stream_check(int device, void* stream) {
+  static std::mutex mu[16];            // of each device's second word
+  KqhDevice dev;
+  const int rc = kqh_device(device, &dev);
+  if (rc) return rc;
+  const cudaStream_t s = (cudaStream_t)stream;
+  CU(cudaStreamSynchronize(s));        // the long wait, without the lock
+  int e = 0;
+  {
+    std::lock_guard<std::mutex> lk(mu[device]);
+    k_take_flags<<<1, 1, 0, s>>>(dev.err, dev.err + 1);
+    CU(cudaGetLastError());
+    CU(cudaMemcpyAsync(&e, dev.err + 1, sizeof(int), cudaMemcpyDeviceToHost, s));
+    CU(cudaStreamSynchronize(s));
+  }
+  return e ? kqh_error(KQ_ERR_ARG, "an operator met device operands out of range:" + kqh_operands(e)) : KQ_OK;
 }

@@ -56,3 +56,62 @@ def test_clusters_whose_last_blocks_have_little_to_do(env, vocab, kind):
         want[:, :n] = torch.where(z.float() == top, torch.arange(vocab, device="cuda", dtype=torch.int32), vocab).amin(2)
         K.check_stream()
         assert torch.equal(ids[:, :n], want[:, :n]) and torch.equal(out, z)
+
+
+def test_flags_of_several_streams_are_all_reported(env):
+    """Checks on one stream while others raise flags: each kind of flag is reported, none is lost."""
+    K, torch = env
+    t = dict(dtype=torch.int32, device="cuda")
+    z, row = torch.zeros((1, 64), device="cuda"), torch.tensor([7], **t)
+    out, mask = torch.empty_like(z), torch.zeros((1, 2), **t)
+    k = torch.zeros((1, 1, 16, 64), device="cuda", dtype=torch.float16)
+    cache, q, table, lens = K.PagedCache(k, k), torch.zeros((1, 1, 64), device="cuda"), torch.tensor([[3]], **t), torch.tensor([5], **t)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    K.check_stream()
+    for _ in range(20):
+        K.logit_rules(z, out, mask=mask, mask_row=row, stream=a.cuda_stream)
+        cache.attend(q, table, lens, torch.empty_like(q), stream=b.cuda_stream)
+        texts = []
+        for s in (a, b):
+            try:
+                K.check_stream(stream=s.cuda_stream)
+            except ValueError as e:
+                texts.append(str(e))
+        assert "row index" in " ".join(texts) and "page id" in " ".join(texts)
+        K.check_stream()
+
+
+def test_two_threads(env):
+    """Operators of two host threads, each on a stream and a cache of its own."""
+    import threading
+    K, torch = env
+    g = torch.Generator(device="cuda").manual_seed(21)
+    t = dict(dtype=torch.int32, device="cuda")
+    k, v = (torch.randn((64, 2, 16, 128), device="cuda", generator=g).half() for _ in range(2))
+    table = torch.arange(64, **t).view(2, 32)
+    lens = torch.tensor([500, 77], **t)
+    q = torch.randn((2, 8, 128), device="cuda", generator=g)
+    z = torch.randn((2, 5000), device="cuda", generator=g)
+    ref = K.PagedCache(k, v).attend(q, table, lens, torch.empty_like(q))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            cache, out, o2, best = K.PagedCache(k, v), torch.empty_like(q), torch.empty_like(z), torch.zeros(2, **t)
+            for _ in range(200):
+                cache.attend(q, table, lens, out, stream=s.cuda_stream)
+                K.logit_rules(z, o2, best=best, stream=s.cuda_stream)
+            s.synchronize()
+            if not (torch.equal(out, ref) and torch.equal(o2, z) and torch.equal(best, z.argmax(1).int())):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not wrong
+    K.check_stream()

@@ -70,3 +70,25 @@ def test_caches_made_on_a_used_engine_while_the_default_stream_is_busy(env, kind
         return got
 
     assert ids(True) == ids(False)
+
+
+def test_a_step_reports_its_own_flags_alone(env):
+    K, torch = env
+    t = dict(dtype=torch.int32, device="cuda")
+    e = engine(K, n_layers=1)
+    e.paged_caches(4, 16, max_seq=2)
+    table = np.arange(4).reshape(2, 2)
+    step = (table, [0, 1], [5, 6], [0, 0])
+    ids = e.paged_step(*step)
+    K.check_stream()
+    z = torch.zeros((1, 64), device="cuda")
+    K.logit_rules(z, torch.empty_like(z), mask=torch.zeros((1, 2), **t), mask_row=torch.tensor([7], **t))
+    assert e.paged_step(*step) == ids                    # another caller's flag is not the step's
+    with pytest.raises(ValueError, match="row index"):
+        K.check_stream()                                 # and is kept for that caller
+    mask = torch.full((1, CFG["vocab"] // 32), -1, **t)
+    with pytest.raises(ValueError, match="row index"):
+        e.paged_step(*step, rules=dict(mask=mask, mask_row=torch.tensor([0, 3], **t)))
+    K.check_stream()                                     # the step's flag was the step's
+    assert e.paged_step(*step, rules=dict(mask=mask, mask_row=torch.tensor([0, -1], **t))) == ids
+    e.close()
