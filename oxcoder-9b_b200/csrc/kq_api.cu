@@ -2541,6 +2541,12 @@ extern "C" int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int m
   if ((rc = verify_buffers(m)) || (rc = batch_buffers(m))) return rc;
   cudaStream_t s = m->stream;
   const int M = n;
+  kq_rule_args R;   // what is wrong with the rules is said before any token is fed
+  std::memset(&R, 0, sizeof(R));
+  if (rules) R = *rules;
+  R.logits = m->vlogits; R.out = m->vlogits; R.in_ld = R.out_ld = c.vocab; R.best = m->out_ids;
+  R.n = M; R.vocab = c.vocab; R.type = KQ_F32;
+  if (out && (rc = kqh_rules_check(&R))) return rc;
   kq_model::MetaSlot* ms = nullptr;
   if ((rc = meta_acquire(m, &ms))) return rc;
   for (int i = 0; i < M; ++i) {
@@ -2592,16 +2598,10 @@ extern "C" int kq_paged_step(kq_model* m, const int32_t* table, int n_seq, int m
     SegSpec sh[1] = {{m->out, EPI_F32, m->vlogits, nullptr}};
     if ((rc = launch_tmm(m, sh, 1, m->bxd, m->bxs_n, m->bxd_sum, c.vocab, B))) return rc;
     prof_mark(m, PC_OTHER);
-    kq_rule_args R;
     if (rules) {
-      R = *rules;
       CU(cudaEventRecord(m->pev_in, (cudaStream_t)stream));
       CU(cudaStreamWaitEvent(s, m->pev_in, 0));
-    } else {
-      std::memset(&R, 0, sizeof(R));
     }
-    R.logits = m->vlogits; R.out = m->vlogits; R.in_ld = R.out_ld = c.vocab; R.best = m->out_ids;
-    R.n = M; R.vocab = c.vocab; R.type = KQ_F32;
     if ((rc = kqh_logit_rules(&R, m->device, m->err, s))) return rc;
   }
   prof_mark(m, PC_END);

@@ -21,5 +21,6 @@ struct kq_pages;
 // kq_pages_create with another handle's attention scratch (null: its own): the handles' calls share a stream,
 // and `with` is freed last.
 kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with, int* err);
-// kq_logit_rules (a kq_rule_args).
+// kq_logit_rules (a kq_rule_args); its checks of the arguments alone.
+int kqh_rules_check(const void* args);
 int kqh_logit_rules(const void* args, int device, int* err, void* stream);

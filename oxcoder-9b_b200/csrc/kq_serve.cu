@@ -323,7 +323,7 @@ static int rules_setup(int device) {
   return KQ_OK;
 }
 
-int kqh_logit_rules(const void* args, int device, int* err, void* stream) {
+int kqh_rules_check(const void* args) {
   const kq_rule_args* a = static_cast<const kq_rule_args*>(args);
   REQUIRE(a, "kq_logit_rules: null argument");
   REQUIRE(a->n >= 0 && a->vocab >= 1 && a->vocab <= KQ_RULES_MAX_VOCAB && a->n <= (1 << 26), "kq_logit_rules: bad row count or vocabulary size");
@@ -337,9 +337,13 @@ int kqh_logit_rules(const void* args, int device, int* err, void* stream) {
   REQUIRE(!a->bias_id == !a->bias && (a->bias ? (a->n_bias >= 0 && a->bias_ld >= a->n_bias) : a->n_bias == 0), "kq_logit_rules: bad bias lists");
   REQUIRE(a->mask ? (a->n_masks >= 1 && a->mask_ld >= (a->vocab + 31) / 32 && (a->mask_row || a->n <= a->n_masks)) : !a->mask_row,
           "kq_logit_rules: bad masks");
+  return KQ_OK;
+}
+int kqh_logit_rules(const void* args, int device, int* err, void* stream) {
+  const kq_rule_args* a = static_cast<const kq_rule_args*>(args);
   KqhDevice dev;
-  int rc = kqh_device(device, &dev);
-  if (rc || a->n == 0) return rc;
+  int rc = kqh_rules_check(a);
+  if (rc || (rc = kqh_device(device, &dev)) || a->n == 0) return rc;
   RuleParams P;
   P.in = a->logits; P.out = a->out; P.in_ld = a->in_ld; P.out_ld = a->out_ld; P.best = a->best;
   P.hist = a->hist; P.hist_len = a->hist_len; P.prompt_len = a->prompt_len; P.hist_ld = a->hist_ld;
@@ -351,7 +355,7 @@ int kqh_logit_rules(const void* args, int device, int* err, void* stream) {
   // 32-bit counts only where a history may hold more of one id than 14 bits count. The smallest
   // cluster whose CTAs hold at most RL_BYTES, then larger ones while the device has CTAs to spare.
   const bool deep = a->max_hist > (int)RlCount<false>::MOST;
-  const int vec = 16 / es, reach = a->vocab + vec - 1, bytes = !P.hist && !P.n_bias ? 0 : deep ? 4 : 2;
+  const int vec = 16 / type_size(a->type), reach = a->vocab + vec - 1, bytes = !P.hist && !P.n_bias ? 0 : deep ? 4 : 2;
   int cl = 1;
   while (cl < RL_CLUSTER && ((long long)reach * bytes > (long long)cl * RL_BYTES ||
                              ((long long)a->n * cl * 2 <= 2 * dev.nsm && reach > cl * RL_THREADS * vec)))
