@@ -18,8 +18,7 @@ std::string kqh_operands(int bits);
 // A model's operators leave their flags in its own error word (`err`), which its own steps read: the flags of
 // other callers on the device stay theirs.
 struct kq_pages;
-// kq_pages_create with another handle's attention scratch (null: its own): the handles' calls share a stream,
-// and `with` is freed last.
+// kq_pages_create with another handle's attention scratch (null: its own): the handles' calls share a stream.
 kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with, int* err);
 // kq_logit_rules (a kq_rule_args); its checks of the arguments alone.
 int kqh_rules_check(const void* args);

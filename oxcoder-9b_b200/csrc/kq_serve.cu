@@ -25,12 +25,19 @@ using namespace kq;
     if (!(cond)) return kqh_error(KQ_ERR_ARG, (text));   \
   } while (0)
 
+// The attention's scratch of a handle, or of several whose calls share a stream.
+struct Scratch {
+  AttendScratch s{};
+  int device = 0;
+  std::atomic<int> users{1};
+  Scratch* next = nullptr;
+};
+
 struct kq_pages {
   kq_page_desc d{};
   int device = 0, shift = 0;
   KqhDevice dev{};
-  AttendScratch scratch{};
-  bool shared = false;   // the scratch belongs to another handle
+  Scratch* scratch = nullptr;
 };
 
 // The attention kernel of a cache type, head size, query heads per CTA (8 or 16) and precision.
@@ -110,47 +117,80 @@ static int pages_check(const kq_page_desc* d) {
   return KQ_OK;
 }
 
-// Scratches of freed handles, kept for the next ones: a server makes and drops handles while it runs, and an
+// Scratches of freed handles are kept for the next ones: a server makes and drops handles while it runs, and an
 // allocation and its release cost a millisecond and a synchronisation each. Between launches a scratch's
-// tickets are zero, so it can be handed on as it is.
+// tickets are zero, so it can be handed on as it is. Launches may still use a scratch when its last user leaves, so
+// it only becomes idle when a new handle finds none that is, and waits for the device: leaving makes no CUDA
+// call, for it may happen at any time (a collected Python object, in the middle of a capture).
 constexpr size_t SCRATCH_PART = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
-constexpr int SCRATCH_KEEP = 4;      // per device
+constexpr int SCRATCH_KEEP = 16;     // idle ones per device; the rest are released at that time
 static std::mutex g_scratch_mu;
-static struct { AttendScratch s[SCRATCH_KEEP]; int n; } g_scratch[16];
+static struct { Scratch *idle, *left; } g_scratch[16];
 
-static cudaError_t scratch_take(int device, AttendScratch& out) {
+static cudaError_t scratch_take(int device, Scratch*& out) {
+  Scratch* left;
   {
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     auto& kept = g_scratch[device];
-    if (kept.n) {
-      out = kept.s[--kept.n];
+    if ((out = kept.idle)) {
+      kept.idle = out->next;
+      out->users = 1;
       return cudaSuccess;
     }
+    left = kept.left;
+    kept.left = nullptr;
   }
+  if (left) {
+    const cudaError_t e = cudaDeviceSynchronize();      // no launch uses these any more
+    Scratch* rest = nullptr;
+    {
+      std::lock_guard<std::mutex> lk(g_scratch_mu);
+      auto& kept = g_scratch[device];
+      int n = 0;
+      for (Scratch* s = kept.idle; s; s = s->next) ++n;
+      if (e == cudaSuccess) {
+        out = left;
+        left = left->next;
+        out->users = 1;
+      }
+      while (left) {
+        Scratch* s = left;
+        left = s->next;
+        Scratch*& list = e != cudaSuccess ? kept.left : n++ < SCRATCH_KEEP ? kept.idle : rest;
+        s->next = list;
+        list = s;
+      }
+    }
+    while (rest) {
+      Scratch* s = rest;
+      rest = s->next;
+      cudaFree(s->s.part);
+      delete s;
+    }
+    return e;
+  }
+  if (!(out = new (std::nothrow) Scratch)) return cudaErrorMemoryAllocation;
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, SCRATCH_PART + PA_MAX_CTAS * sizeof(int));
-  if (e != cudaSuccess) return e;
-  out.part = static_cast<float*>(p);
-  out.ticket = reinterpret_cast<int*>(static_cast<char*>(p) + SCRATCH_PART);
-  e = cudaMemset(out.ticket, 0, PA_MAX_CTAS * sizeof(int));
-  if (e == cudaSuccess) e = cudaStreamSynchronize(0);   // the first call may be on a stream that does not wait for this one
+  if (e == cudaSuccess) {
+    out->device = device;
+    out->s.part = static_cast<float*>(p);
+    out->s.ticket = reinterpret_cast<int*>(static_cast<char*>(p) + SCRATCH_PART);
+    e = cudaMemset(out->s.ticket, 0, PA_MAX_CTAS * sizeof(int));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(0);   // the first call may be on a stream that does not wait for this one
+  }
   if (e != cudaSuccess) {
     cudaFree(p);
-    out = AttendScratch{};
+    delete out;
+    out = nullptr;
   }
   return e;
 }
-static void scratch_give(int device, const AttendScratch& s) {
-  if (cudaSetDevice(device) != cudaSuccess) return;
-  if (cudaDeviceSynchronize() == cudaSuccess) {         // no launch still uses it
-    std::lock_guard<std::mutex> lk(g_scratch_mu);
-    auto& kept = g_scratch[device];
-    if (kept.n < SCRATCH_KEEP) {
-      kept.s[kept.n++] = s;
-      return;
-    }
-  }
-  cudaFree(s.part);
+static void scratch_leave(Scratch* s) {
+  if (--s->users) return;
+  std::lock_guard<std::mutex> lk(g_scratch_mu);
+  s->next = g_scratch[s->device].left;
+  g_scratch[s->device].left = s;
 }
 // The attention kernels' shared memory, allowed once per device (which is current).
 static cudaError_t attend_setup(int device, int type, int hd) {
@@ -192,7 +232,7 @@ kq_pages* kqh_pages_create(const void* desc, int device, const kq_pages* with, i
   cudaError_t e = attend_setup(device, d->type, d->head_dim);
   if (e == cudaSuccess && with) {
     c->scratch = with->scratch;
-    c->shared = true;
+    ++c->scratch->users;
   } else if (e == cudaSuccess) {
     e = scratch_take(device, c->scratch);
   }
@@ -209,7 +249,7 @@ extern "C" kq_pages* kq_pages_create(const kq_page_desc* d, int device) { return
 
 extern "C" void kq_pages_free(kq_pages* c) {
   if (!c) return;
-  if (c->scratch.part && !c->shared) scratch_give(c->device, c->scratch);
+  if (c->scratch) scratch_leave(c->scratch);
   delete c;
 }
 
@@ -299,7 +339,7 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* st
   const long long tiles = (((long long)a->max_pages << c->shift) + PA_TILE - 1) / PA_TILE;
   const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
   const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * k.per_sm));
-  CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, 1, P, c->scratch));
+  CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, 1, P, c->scratch->s));
   return KQ_OK;
 }
 

@@ -115,3 +115,53 @@ def test_two_threads(env):
         x.join()
     assert not wrong
     K.check_stream()
+
+
+def pool(torch, seed, pages=64):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    k, v = (torch.randn((pages, 2, 16, 128), device="cuda", generator=g).half() for _ in range(2))
+    return k, v, torch.randn((1, 8, 128), device="cuda", generator=g)
+
+
+def plain(torch, k, v, q, L):
+    """Attention of one token over the first L positions of pages 0, 1, ... in 64 bits."""
+    kk, vv = (x.double().transpose(0, 1).reshape(x.shape[1], -1, x.shape[3])[:, :L] for x in (k, v))
+    z = torch.einsum("ghd,gtd->ght", q[0].double().view(k.shape[1], -1, q.shape[2]), kk) / q.shape[2] ** 0.5
+    return torch.einsum("ght,gtd->ghd", z.softmax(-1), vv).reshape(q.shape[1:])
+
+
+def test_handles_close_at_any_time(env):
+    """During a capture, and while the device is busy: closing waits for nothing and calls nothing that a capture forbids."""
+    K, torch = env
+    k, v, q = pool(torch, 41)
+    table, lens = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64), torch.tensor([1000], dtype=torch.int32, device="cuda")
+    want = plain(torch, k, v, q, 1000)
+    caches = [K.PagedCache(k, v) for _ in range(24)]
+    outs = [torch.empty_like(q) for _ in caches]
+    for c, o in zip(caches, outs):
+        c.attend(q, table, lens, o)
+    x = torch.randn((4096, 4096), device="cuda")
+    for _ in range(200):                                 # some tens of milliseconds
+        x = (x @ x).clamp_(-1, 1)
+    late = torch.empty_like(q)
+    caches[0].attend(q, table, lens, late)
+    done = torch.cuda.Event()
+    done.record()
+    for c in caches[:12]:
+        c.close()
+    assert not done.query()
+    torch.cuda.synchronize()
+    s, graph, again = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph, stream=s):
+        caches[23].attend(q, table, lens, again, stream=s.cuda_stream)
+        for c in caches[12:23]:
+            c.close()
+    graph.replay()
+    fresh = [K.PagedCache(k, v) for _ in range(24)]      # the first waits for the device
+    more = [torch.empty_like(q) for _ in fresh]
+    for c, o in zip(fresh, more):
+        c.attend(q, table, lens, o)
+    K.check_stream()
+    for o in outs + more + [late, again]:
+        assert float((o[0].double() - want).abs().max()) < 1e-5    # weights of 22 bits over unit normal values
+        assert torch.equal(o, outs[0])
