@@ -192,6 +192,24 @@ static void scratch_leave(Scratch* s) {
   s->next = g_scratch[s->device].left;
   g_scratch[s->device].left = s;
 }
+// A graph under capture on `stream` uses the scratch for as long as the graph, or what was instantiated from it, lives.
+static cudaError_t scratch_hold(Scratch* s, cudaStream_t stream) {
+  cudaStreamCaptureStatus state;
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaStreamGetCaptureInfo(stream, &state, nullptr, &graph);
+  if (e != cudaSuccess || state != cudaStreamCaptureStatusActive) return e;
+  cudaUserObject_t held;
+  ++s->users;
+  e = cudaUserObjectCreate(&held, s, [](void* p) { scratch_leave(static_cast<Scratch*>(p)); }, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    --s->users;
+    return e;
+  }
+  e = cudaGraphRetainUserObject(graph, held, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) cudaUserObjectRelease(held, 1);
+  return e;
+}
+
 // The attention kernels' shared memory, allowed once per device (which is current).
 static cudaError_t attend_setup(int device, int type, int hd) {
   static std::atomic<unsigned> done[16];
@@ -339,6 +357,7 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* st
   const long long tiles = (((long long)a->max_pages << c->shift) + PA_TILE - 1) / PA_TILE;
   const long long most = (long long)a->n * P.n_kv * ((G + heads - 1) / heads) * tiles;
   const unsigned grid = (unsigned)std::min<long long>(most, std::min(PA_MAX_CTAS, c->dev.nsm * k.per_sm));
+  CU(scratch_hold(c->scratch, (cudaStream_t)stream));
   CU(launch(k.fn, dim3(grid), PA_WARPS * 32, k.smem, stream, 1, P, c->scratch->s));
   return KQ_OK;
 }

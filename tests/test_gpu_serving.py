@@ -165,3 +165,55 @@ def test_handles_close_at_any_time(env):
     for o in outs + more + [late, again]:
         assert float((o[0].double() - want).abs().max()) < 1e-5    # weights of 22 bits over unit normal values
         assert torch.equal(o, outs[0])
+
+
+def test_graphs_keep_the_scratch_of_closed_handles(env):
+    """Replays of a graph whose handle is gone, beside calls of handles made since: each has a scratch of its own."""
+    K, torch = env
+    k, v, q = pool(torch, 43)
+    table, lens = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64), torch.tensor([1000], dtype=torch.int32, device="cuda")
+    want = plain(torch, k, v, q, 1000)
+    s, o = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        graphs, outs = [], [torch.empty_like(q) for _ in range(4)]
+        for out in outs:
+            cache = K.PagedCache(k, v)
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                cache.attend(q, table, lens, out, stream=s.cuda_stream)
+            cache.close()
+        caches = [K.PagedCache(k, v) for _ in range(4)]
+        more = [torch.empty_like(q) for _ in caches]
+        torch.cuda.synchronize()
+        for i in range(50):
+            with torch.cuda.stream(s):
+                graphs[i % 4].replay()
+            caches[i % 4].attend(q, table, lens, more[i % 4], stream=o.cuda_stream)
+        torch.cuda.synchronize()
+        K.check_stream()
+        for x in outs + more:
+            assert float((x[0].double() - want).abs().max()) < 1e-5
+            assert torch.equal(x, outs[0])
+        del graphs
+        for c in caches:
+            c.close()
+
+
+def test_scratches_of_dropped_graphs_come_back(env):
+    """40 handles captured, closed and their graphs dropped, one after another: not 40 scratches of 10 MB."""
+    K, torch = env
+    k, v, q = pool(torch, 44)
+    table, lens = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64), torch.tensor([300], dtype=torch.int32, device="cuda")
+    s, out = torch.cuda.Stream(), torch.empty_like(q)
+    free = []
+    for i in range(44):
+        cache, graph = K.PagedCache(k, v), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            cache.attend(q, table, lens, out, stream=s.cuda_stream)
+        graph.replay()
+        cache.close()
+        torch.cuda.synchronize()
+        del graph
+        if i in (3, 43):
+            free.append(torch.cuda.mem_get_info()[0])
+    assert free[0] - free[1] < 200 << 20
