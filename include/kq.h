@@ -373,6 +373,10 @@ int kq_logit_rules(const kq_rule_args* a, int device, void* stream);   /* the fi
  * whose message says what is wrong. */
 #define KQ_TENSOR_OTHER 1
 int kq_tensor_source(int (*describe)(void* object, void* dl_tensor));
+/* The stream that the binding's own operations on a device are enqueued on now (DLPack's current_work_stream; device_type 2:
+ * CUDA): the kq_*_tensors calls ask for it where `stream` is KQ_STREAM_CURRENT. None named: the legacy default. */
+#define KQ_STREAM_CURRENT ((void*)-1)
+int kq_tensor_stream(int (*current)(int device_type, int32_t device, void** stream));
 int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table, void* pos, void* seq, void* cos_t, void* sin_t, void* q,
                            void* q_out, void* stream);
 int kq_page_attend_tensors(kq_pages* c, void* q, void* table, void* len, void* out, void* seq, int window, float scale, void* stream);

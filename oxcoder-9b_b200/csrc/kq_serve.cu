@@ -448,6 +448,21 @@ extern "C" int kq_tensor_source(int (*describe)(void*, void*)) {
   return KQ_OK;
 }
 
+typedef int (*CurrentFn)(int, int32_t, void**);
+static std::atomic<CurrentFn> g_current;
+
+extern "C" int kq_tensor_stream(int (*current)(int, int32_t, void**)) {
+  g_current.store(current, std::memory_order_release);
+  return KQ_OK;
+}
+// `stream`, or the binding's current one on the device where that is asked for.
+static bool stream_for(int device, void*& stream) {
+  if (stream != KQ_STREAM_CURRENT) return true;
+  stream = nullptr;
+  const CurrentFn current = g_current.load(std::memory_order_acquire);
+  return !current || current(2, device, &stream) == 0;
+}
+
 constexpr int T_I32 = 100;
 struct Tensor {
   void* p = nullptr;
@@ -486,7 +501,7 @@ static bool vector_as(void* object, int type, int device, long long n, Tensor& t
 
 extern "C" int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table, void* pos, void* seq, void* cos_t, void* sin_t,
                                       void* q, void* q_out, void* stream) {
-  FITS(c && !cos_t == !sin_t && !q == !q_out);
+  FITS(c && !cos_t == !sin_t && !q == !q_out && stream_for(c->device, stream));
   const int dev = c->device;
   Tensor tk, tv, tt, tp, ts, tc, tsn, tq, to;
   FITS(tensor_of(k, 3, tk) && tk.device == dev && tk.n[1] == c->d.n_kv_heads && tk.n[2] == c->d.head_dim && tensor_as(v, tk, tv, 3));
@@ -515,7 +530,7 @@ extern "C" int kq_page_append_tensors(kq_pages* c, void* k, void* v, void* table
 
 extern "C" int kq_page_attend_tensors(kq_pages* c, void* q, void* table, void* len, void* out, void* seq, int window, float scale,
                                       void* stream) {
-  FITS(c);
+  FITS(c && stream_for(c->device, stream));
   const int dev = c->device;
   Tensor tq, to, tt, tl, ts;
   FITS(tensor_of(q, 3, tq) && tq.device == dev && tq.n[2] == c->d.head_dim && tensor_as(out, tq, to, 3));
@@ -541,6 +556,7 @@ extern "C" int kq_logit_rules_tensors(void* logits, void* out, void* best, void*
   FITS(tensor_of(logits, 2, tl) && tensor_as(out, tl, to, 2));
   const int dev = tl.device;
   const long long n = tl.n[0];
+  FITS(stream_for(dev, stream));
   if (best) FITS(vector_as(best, T_I32, dev, n, tb));
   if (hist) FITS(tensor_of(hist, 2, th) && th.type == T_I32 && th.device == dev && th.n[0] == n && vector_as(hist_len, T_I32, dev, n, thl));
   if (prompt_len) FITS(vector_as(prompt_len, T_I32, dev, n, tp));

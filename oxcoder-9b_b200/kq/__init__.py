@@ -108,6 +108,7 @@ SIGNATURES = {
     "kq_paged_caches": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
     "kq_paged_step": (C.c_int, [C.c_void_p, PI32, C.c_int, C.c_int, PI32, PI32, PI32, C.c_int, C.c_char_p, C.c_void_p, PI32]),
     "kq_tensor_source": (C.c_int, [C.c_void_p]),
+    "kq_tensor_stream": (C.c_int, [C.c_void_p]),
     "kq_page_append_tensors": (C.c_int, [C.c_void_p] * 11),
     "kq_page_attend_tensors": (C.c_int, [C.c_void_p] * 6 + [C.c_int, C.c_float, C.c_void_p]),
     "kq_logit_rules_tensors": (C.c_int, [C.c_void_p] * 14),
@@ -428,12 +429,12 @@ class Engine(object):
         """Allocate the (zeroed) page pool: n_pages pages of `page` positions per layer, shared by all sequences."""
         check(lib().kq_paged_caches(self.h, int(n_pages), int(page), int(max_seq)))
 
-    def paged_step(self, table, seqs, toks, pos, pick=True, rules=None, stream=0):
+    def paged_step(self, table, seqs, toks, pos, pick=True, rules=None, stream=None):
         """Tokens toks[i] at positions pos[i] of the sequences with page-table rows seqs[i] (table: host
         [sequences, pages], the pages the caller gave each): a decode step, a prompt chunk or both. Returns
         the greedy ids (pick=False: None, the tokens are only fed). rules: kq.logit_rules' history, penalties,
-        biases and masks as a dict of device tensors with a row per token, ready on `stream`; a row whose
-        rules allow nothing gives -1."""
+        biases and masks as a dict of device tensors with a row per token, ready on `stream` (None: PyTorch's
+        current stream); a row whose rules allow nothing gives -1."""
         from . import serve
         tb = np.ascontiguousarray(table, np.int32)
         sq, t, p = (np.ascontiguousarray(a, np.int32) for a in (seqs, toks, pos))
@@ -441,6 +442,8 @@ class Engine(object):
             raise ValueError("the page table must be [sequences, pages], seqs, toks and pos of one length")
         out = np.empty(len(t), np.int32) if pick or rules is not None else None
         packed = None if rules is None else serve.pack_rules(len(t), self.vocab, self.device, **rules)
+        if stream is None:
+            stream = serve.current_stream(self.device, *rules.values()) if rules else 0
         check(lib().kq_paged_step(self.h, _ptr(tb, PI32), tb.shape[0], tb.shape[1], _ptr(sq, PI32), _ptr(t, PI32), _ptr(p, PI32),
                                   len(t), packed, stream, None if out is None else _ptr(out, PI32)))
         return None if out is None else [int(v) for v in out]

@@ -7,11 +7,13 @@
     kq.check_stream()                               # waits, raises what the kernels flagged
 
 Tensors are any objects with PyTorch's tensor interface (data_ptr, shape, stride, dtype, get_device);
-this module does not import it. Calls are enqueued on `stream` (a CUDA stream handle, 0 = legacy
-default) and neither wait nor allocate. Wrong types, shapes, strides or devices raise ValueError
-before anything is launched."""
+this module does not import it. Calls are enqueued on `stream`, a CUDA stream handle (0: the legacy default
+stream; None: the stream that PyTorch's own operations are enqueued on at the time, the legacy default where the
+tensors' library does not tell), and neither wait nor allocate. Wrong types, shapes, strides or devices
+raise ValueError before anything is launched."""
 import ctypes as C
 import struct
+import sys
 
 F32, F16, BF16, E4M3, I32 = 0, 1, 2, 3, 4
 _NAMES = {"float32": F32, "float16": F16, "bfloat16": BF16, "float8_e4m3fn": E4M3, "int32": I32, "uint32": I32}
@@ -27,7 +29,9 @@ class _Direct(object):
     interface, or None of them: those calls answer OTHER for whatever they cannot take, and the checks
     below then say why. They keep Python's lock (the interface needs it)."""
     OTHER = 1
+    CURRENT = C.c_void_p(-1).value                      # KQ_STREAM_CURRENT
     type = None
+    current = None
     _tried = set()
 
     @classmethod
@@ -45,16 +49,32 @@ class _Direct(object):
         if C.c_uint32.from_address(api).value != 1:     # the interface's major version
             return
         describe = C.c_void_p.from_address(api + 5 * 8).value   # dltensor_from_py_object_no_sync
-        if not describe:
+        current = C.c_void_p.from_address(api + 6 * 8).value    # current_work_stream
+        if not describe or not current:
             return
         lib = C.PyDLL(LIB_PATH)
         lib.kq_tensor_source.argtypes = [C.c_void_p]
         lib.kq_tensor_source(describe)
+        lib.kq_tensor_stream.argtypes = [C.c_void_p]
+        lib.kq_tensor_stream(current)
+        cls.current = C.PYFUNCTYPE(C.c_int, C.c_int, C.c_int32, C.POINTER(C.c_void_p))(current)
         for name in ("kq_page_append_tensors", "kq_page_attend_tensors", "kq_logit_rules_tensors"):
             f = getattr(lib, name)
             f.restype, f.argtypes = SIGNATURES[name]
             setattr(cls, name[3:-8], f)
         cls.type = t
+
+
+def current_stream(device, *tensors):
+    """Handle of the stream on which the library of such tensors enqueues its operations on the device now (0: unknown)."""
+    for t in tensors:
+        if t is not None:
+            _Direct.try_type(type(t))
+    if _Direct.current is not None:
+        s = C.c_void_p()
+        return s.value or 0 if _Direct.current(2, device, C.byref(s)) == 0 else 0
+    torch = sys.modules.get("torch")                    # a PyTorch without that interface
+    return torch.cuda.current_stream(device).cuda_stream if torch is not None and torch.cuda.is_initialized() else 0
 
 
 def _bind():
@@ -165,7 +185,7 @@ class PagedCache(object):
             raise ValueError("more tokens than page-table rows: give seq")
         return t, 0, s[0] if n_seq > 1 else wide, n_seq, wide
 
-    def append(self, k, v, table, pos, seq=None, rope=None, q=None, q_out=None, stream=0):
+    def append(self, k, v, table, pos, seq=None, rope=None, q=None, q_out=None, stream=None):
         """K/V rows k, v [n, n_kv_heads, head_dim] (fp32, fp16 or bf16) to positions pos [n] of the sequences whose
         page-table rows are seq [n] (None: row i for token i); table [sequences, pages] int32. rope: (cos, sin)
         fp32 [positions, rot / 2]: the keys are rotated on the way, and so are the queries q [n, heads,
@@ -178,7 +198,8 @@ class PagedCache(object):
                 and (q is None or (type(q) is T and type(q_out) is T)):
             rc = _Direct.page_append(self.h, id(k), id(v), id(table), id(pos), None if seq is None else id(seq),
                                      None if rope is None else id(rope[0]), None if rope is None else id(rope[1]),
-                                     None if q is None else id(q), None if q_out is None else id(q_out), stream)
+                                     None if q is None else id(q), None if q_out is None else id(q_out),
+                                     _Direct.CURRENT if stream is None else stream)
             if not rc:
                 return
             if rc != _Direct.OTHER:
@@ -212,12 +233,14 @@ class PagedCache(object):
             raise ValueError("q_out without q")
         if not n:
             return
+        if stream is None:
+            stream = current_stream(dev, k)
         rc = self._append(self.h, _APPEND.pack(kp, vp, qp, op, k0, k1, v0, v1, q0, q1, o0, o1, tp, sp, pp, cp, np_, ld, rl, n,
                                                heads, kind, n_seq, wide, rot, n_pos), stream)
         if rc:
             self._check(rc)
 
-    def attend(self, q, table, lens, out, seq=None, window=0, scale=None, stream=0):
+    def attend(self, q, table, lens, out, seq=None, window=0, scale=None, stream=None):
         """out[i][h] = softmax(scale q[i][h] . K) V over positions [0, lens[i]) of the sequence with page-table row
         seq[i] (None: row i); window > 0: over its last `window` positions. q, out [n, heads, head_dim] of one
         type (fp32, fp16, bf16), scale: 1 / sqrt(head_dim) by default. A row without positions gives zeros."""
@@ -226,7 +249,7 @@ class PagedCache(object):
         T = _Direct.type
         if type(q) is T and type(table) is T and type(lens) is T and type(out) is T and (seq is None or type(seq) is T):
             rc = _Direct.page_attend(self.h, id(q), id(table), id(lens), id(out), None if seq is None else id(seq), window,
-                                     self.hd ** -0.5 if scale is None else scale, stream)
+                                     self.hd ** -0.5 if scale is None else scale, _Direct.CURRENT if stream is None else stream)
             if not rc:
                 return out
             if rc != _Direct.OTHER:
@@ -242,6 +265,8 @@ class PagedCache(object):
         lp = _vec(lens, "lens", I32, (n,), dev)
         if not n:
             return out
+        if stream is None:
+            stream = current_stream(dev, q)
         rc = self._attend(self.h, _ATTEND.pack(qp, op, q0, q1, o0, o1, tp, sp, lp, ld, n, heads, kind, n_seq, wide, window,
                                                hd ** -0.5 if scale is None else scale), stream)
         if rc:
@@ -307,7 +332,7 @@ def pack_rules(n, vocab, device, **rules):
 
 
 def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=None, repetition=None, frequency=None,
-                presence=None, bias_ids=None, bias=None, mask=None, mask_row=None, stream=0):
+                presence=None, bias_ids=None, bias=None, mask=None, mask_row=None, stream=None):
     """Penalties for repeated tokens, biases and grammar masks on logits [n, vocab] (fp32, fp16, bf16), into out
     (may be logits); best [n] int32: the greedy ids (-1 where nothing is allowed). hist [n, most] int32 with
     hist_len [n] tokens in use, of which prompt_len [n] (None: 0) are the prompt; repetition, frequency, presence:
@@ -329,7 +354,7 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
             else:
                 break
         else:
-            rc = _Direct.logit_rules(*ids, stream)
+            rc = _Direct.logit_rules(*ids, _Direct.CURRENT if stream is None else stream)
             if not rc:
                 return out
             if rc != _Direct.OTHER:
@@ -347,14 +372,18 @@ def logit_rules(logits, out, best=None, hist=None, hist_len=None, prompt_len=Non
     fields = _rule_fields(n, vocab, dev, hist, hist_len, prompt_len, repetition, frequency, presence, bias_ids, bias, mask, mask_row)
     if not n:
         return out
+    if stream is None:
+        stream = current_stream(dev, logits)
     rc = _rules()(_RULES.pack(ip, op, ild, old, bp, *fields[:13], n, vocab, kind, *fields[13:]), dev, stream)
     if rc:
         _bind()[1](rc)
     return out
 
 
-def check_stream(device=0, stream=0):
-    """Waits for the stream and raises ValueError if an operator's kernel met a page id, position, length or row
+def check_stream(device=0, stream=None):
+    """Waits for the stream (None: as for the operators) and raises ValueError if an operator's kernel met a page id, position, length or row
     index out of range since the last check on this device (such entries are skipped, never read)."""
     lib, check, _ = _bind()
+    if stream is None:
+        stream = current_stream(device) if lib.kq_device_count() > device else 0
     check(lib.kq_stream_check(device, stream))

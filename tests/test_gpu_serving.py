@@ -217,3 +217,40 @@ def test_scratches_of_dropped_graphs_come_back(env):
         if i in (3, 43):
             free.append(torch.cuda.mem_get_info()[0])
     assert free[0] - free[1] < 200 << 20
+
+
+def test_calls_without_a_stream_follow_the_current_one(env, way):
+    """Behind work that is still queued on PyTorch's current stream, and inside a capture of it."""
+    K, torch = env
+    k, v, q0 = pool(torch, 47)
+    table, lens = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64), torch.tensor([1000], dtype=torch.int32, device="cuda")
+    x, cache, s = torch.randn((4096, 4096), device="cuda"), K.PagedCache(k, v), torch.cuda.Stream()
+    pos, kn = torch.tensor([999], dtype=torch.int32, device="cuda"), torch.empty((1, 2, 128), device="cuda")
+    q, out, z, best = torch.zeros_like(q0), torch.empty_like(q0), torch.zeros((1, 3000), device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(100):                             # some tens of milliseconds
+            x = (x @ x).clamp_(-1, 1)
+        q.copy_(q0)
+        kn.fill_(0.25)
+        z[0, 1234] = 1.0
+        cache.append(kn, kn, table, pos)
+        cache.attend(q, table, lens, out)
+        K.logit_rules(z, z, best=best)
+        K.check_stream()
+    first = out.clone()
+    k[62, :, 7] = v[62, :, 7] = 0.25                     # position 999
+    assert float((first[0].double() - plain(torch, k, v, q0, 1000)).abs().max()) < 1e-5
+    assert best.tolist() == [1234]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        cache.append(kn, kn, table, pos)
+        cache.attend(q, table, lens, out)
+        K.logit_rules(z, z, best=best)
+    q.mul_(0.5)
+    z[0, 77] = 2.0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float((out[0].double() - plain(torch, k, v, q0 * 0.5, 1000)).abs().max()) < 1e-5
+    assert best.tolist() == [77]

@@ -46,7 +46,7 @@ def direct():
         return 0
 
     lib = C.PyDLL(K.LIB_PATH)
-    lib.kq_tensor_source.argtypes = [C.c_void_p]
+    lib.kq_tensor_source.argtypes = lib.kq_tensor_stream.argtypes = [C.c_void_p]
     lib.kq_tensor_source(C.cast(describe, C.c_void_p))
 
     def call(name, *args):
@@ -55,10 +55,12 @@ def direct():
         known.update((id(a), a) for a in args if isinstance(a, Made))
         return f(*(id(a) if isinstance(a, Made) else a for a in args))
 
+    call.lib = lib
     yield call
     was = serve._Direct.type
     serve._Direct.type, serve._Direct._tried = None, set()
     lib.kq_tensor_source(None)
+    lib.kq_tensor_stream(None)
     if was is not None:
         serve._Direct.try_type(was)
 
@@ -76,3 +78,59 @@ def test_masks_too_narrow_for_the_vocabulary_are_not_taken(direct):
     assert rules(direct, mask=Made((2, 7), (5000, 1), INT)) == K.ERR_BACKEND
     for shape, strides in (((2, 6), (5000, 1)), ((2, 6), None), ((2, 1), (7, 1)), ((1, 6), (5000, 1))):
         assert rules(direct, mask=Made(shape, strides, INT), mask_row=Made((2,), kind=INT)) == _Direct.OTHER
+
+
+def test_calls_ask_for_the_current_stream_where_they_are_told_to(direct):
+    """KQ_STREAM_CURRENT: the tensors' library is asked, for the tensors' device; any other handle is taken as it is."""
+    import kq as K
+    from kq.serve import _Direct
+    asked, status = [], [0]
+
+    @C.PYFUNCTYPE(C.c_int, C.c_int, C.c_int32, C.POINTER(C.c_void_p))
+    def current(kind, device, out):
+        asked.append((kind, device))
+        out[0] = 1234
+        return status[0]
+
+    direct.lib.kq_tensor_stream(C.cast(current, C.c_void_p))
+    z = Made((2, 200))
+    none = [None] * 11
+    assert direct("kq_logit_rules_tensors", z, z, *none, 0) == K.ERR_BACKEND and not asked
+    assert direct("kq_logit_rules_tensors", z, z, *none, 77) == K.ERR_BACKEND and not asked
+    assert direct("kq_logit_rules_tensors", z, z, *none, _Direct.CURRENT) == K.ERR_BACKEND and asked == [(2, 0)]
+    status[0] = -1                                       # it does not know: nothing is launched
+    assert direct("kq_logit_rules_tensors", z, z, *none, _Direct.CURRENT) == _Direct.OTHER
+
+
+def test_calls_without_a_stream_take_the_current_one(monkeypatch):
+    """The Python face: what the library is given where no stream is named, both ways of passing tensors."""
+    import kq as K
+    from kq import serve
+    torch = pytest.importorskip("torch")
+    streams = []
+
+    def record(*args):
+        streams.append(args[-1])
+        return 0
+
+    c = object.__new__(K.PagedCache)
+    c.h, c.device, c.n_kv, c.page, c.hd, c.type = 1, -1, 2, 16, 64, serve.F16
+    c._free, c._append, c._attend = (lambda h: None), record, record
+    k, table, i = torch.zeros((1, 2, 64)), torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+
+    def calls(**kw):
+        del streams[:]
+        c.append(k, k, table, i, **kw)
+        c.attend(k, table, i, k, **kw)
+        return streams
+
+    for name in ("page_append", "page_attend"):
+        monkeypatch.setattr(serve._Direct, name, record, raising=False)
+    monkeypatch.setattr(serve._Direct, "type", torch.Tensor)
+    assert calls() == [serve._Direct.CURRENT] * 2
+    assert calls(stream=0) == [0, 0] and calls(stream=5) == [5, 5]
+    monkeypatch.setattr(serve._Direct, "type", None)
+    monkeypatch.setattr(serve, "current_stream", lambda device, *tensors: 99)
+    assert calls() == [99, 99]
+    assert calls(stream=0) == [0, 0] and calls(stream=5) == [5, 5]
+    c.h = None
