@@ -13,25 +13,17 @@ namespace kq {
 
 enum : int { PG_F32 = 0, PG_F16 = 1, PG_BF16 = 2, PG_E4M3 = 3 };   // KQ_F32 .. KQ_E4M3
 
-// x[0] of a row of elements of `type`, as fp32.
-__device__ __forceinline__ float pg_load(const void* row, int type, long long i) {
-  if (type == PG_F32) return reinterpret_cast<const float*>(row)[i];
-  if (type == PG_F16) return __half2float(reinterpret_cast<const __half*>(row)[i]);
-  if (type == PG_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[i]);
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(reinterpret_cast<const __nv_fp8_storage_t*>(row)[i], __NV_E4M3)));
-}
 // Elements i, i + 1 (i even, the row 4-byte aligned at least) of a row of fp32 or 16-bit elements.
 __device__ __forceinline__ float2 pg_load2(const void* row, int type, long long i) {
   if (type == PG_F32) return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(row) + i);
   if (type == PG_F16) return __half22float2(*reinterpret_cast<const __half2*>(reinterpret_cast<const __half*>(row) + i));
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(reinterpret_cast<const __nv_bfloat16*>(row) + i));
 }
-// One rounding of an fp32 value to `type` (8-bit floats saturate at 448; NaN stays NaN).
+// One rounding of an fp32 value to `type` (fp32 or 16 bits).
 __device__ __forceinline__ void pg_store(void* row, int type, long long i, float x) {
   if (type == PG_F32) reinterpret_cast<float*>(row)[i] = x;
   else if (type == PG_F16) reinterpret_cast<__half*>(row)[i] = __float2half_rn(x);
-  else if (type == PG_BF16) reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(x);
-  else reinterpret_cast<__nv_fp8_storage_t*>(row)[i] = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+  else reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(x);
 }
 
 struct PageTable {
@@ -72,7 +64,7 @@ __device__ __forceinline__ void ap_widen(const uint4& a, float (&x)[V]) {
     }
   }
 }
-// V values rounded to type T; p aligned to the V elements.
+// V values rounded to type T (8-bit floats saturate at 448; NaN stays NaN); p aligned to the V elements.
 template <int T, int V>
 __device__ __forceinline__ void ap_store(void* p, const float (&x)[V]) {
   if (T == PG_F32) {
@@ -209,7 +201,7 @@ struct AttendParams {
   const float *ks, *vs;
   PageTable T;
   const int* len;
-  int n, n_heads, n_kv, type, cache_type, window;
+  int n, n_heads, n_kv, type, window;
   float scale;
   int* err;
 };

@@ -312,8 +312,10 @@ extern "C" int kq_page_append(kq_pages* c, const kq_append_args* given, void* st
   P.pos = a->pos; P.cos_t = a->cos_t; P.sin_t = a->sin_t; P.rope_ld = a->rope_ld;
   P.n_heads = a->n_heads; P.n_kv = c->d.n_kv_heads; P.hd = c->d.head_dim;
   P.rot = a->rot; P.n_pos = a->n_pos; P.err = c->dev.err;
-  // up to some waves of CTAs: a head row per thread; more: AP_DEEP rows, the angles read once for all (8192 tokens of
-  // 48 rows 40 against 44.5 us; 1021 tokens of 24 wide rows 10.8 against 9.2)
+  // AP_DEEP head rows a thread above 64 CTAs an SM (the angles are read once for them), one below. Measured in turn, us with
+  // one / three: 48 bf16 rows of 128, 2000 / 4000 / 5000 / 8192 tokens 9.3 / 7.6, 18.7 / 17.9, 24.9 / 25.6, 40.6 / 40.2; 24 fp32
+  // rows of 256, 1000 / 2000 / 3000 / 4000 tokens 7.9 / 7.1, 14.2 / 12.4, 22.1 / 22.9, 29.4 / 31.2. Three are faster while a
+  // call's rows stay in the L2 and up to 7 % slower beyond: the rule costs up to a fifth below its border, 7 % above.
   const int units = c->d.head_dim / (a->src_type == KQ_F32 ? 8 : 16), rows = a->n_heads + 2 * P.n_kv;
   const int slices = (rows * units + AP_THREADS - 1) / AP_THREADS;
   const bool deep = (long long)a->n * slices > 64ll * c->dev.nsm;
@@ -347,7 +349,7 @@ extern "C" int kq_page_attend(kq_pages* c, const kq_attend_args* given, void* st
   P.ks = c->d.k_scale; P.vs = c->d.v_scale;
   P.T = table_of(c, a->table, a->seq, a->table_ld, a->n_seq, a->max_pages);
   P.len = a->len; P.n = a->n; P.n_heads = a->n_heads; P.n_kv = c->d.n_kv_heads; P.type = a->type;
-  P.cache_type = c->d.type; P.window = a->window; P.scale = a->scale; P.err = c->dev.err;
+  P.window = a->window; P.scale = a->scale; P.err = c->dev.err;
   const int G = a->n_heads / P.n_kv;
   // fp32 queries want fp32 scores: the cache's 16-bit type in two or three terms; so do fp16 queries
   // (11 bits) on a bf16 cache (8 bits)
