@@ -25,12 +25,23 @@ using namespace kq;
     if (!(cond)) return kqh_error(KQ_ERR_ARG, (text));   \
   } while (0)
 
-// The attention's scratch of a handle, or of several whose calls share a stream.
+// The attention's scratch of a handle, or of several whose calls share a stream, and of the graphs that captured
+// such calls.
+struct ScratchBlock;
 struct Scratch {
   AttendScratch s{};
   int device = 0;
-  std::atomic<int> users{1};
+  std::atomic<int> users{0};
+  ScratchBlock* block = nullptr;
   Scratch* next = nullptr;
+};
+constexpr int SCRATCH_BLOCK = 4;
+struct ScratchBlock {
+  void* p = nullptr;
+  Scratch s[SCRATCH_BLOCK];
+  int idle = 0;
+  bool released = false;
+  ScratchBlock* next = nullptr;
 };
 
 struct kq_pages {
@@ -117,80 +128,109 @@ static int pages_check(const kq_page_desc* d) {
   return KQ_OK;
 }
 
-// Scratches of freed handles are kept for the next ones: a server makes and drops handles while it runs, and an
-// allocation and its release cost a millisecond and a synchronisation each. Between launches a scratch's
-// tickets are zero, so it can be handed on as it is. Launches may still use a scratch when its last user leaves, so
-// it only becomes idle when a new handle finds none that is, and waits for the device: leaving makes no CUDA
-// call, for it may happen at any time (a collected Python object, in the middle of a capture).
+// Scratches are allocated four at a time, and those of freed handles are kept for the next ones: a server makes and
+// drops handles while it runs, and an allocation costs some milliseconds. Between launches a scratch's tickets are
+// zero, so it can be handed on as it is. Launches may still use a scratch when its last user leaves, and leaving
+// makes no CUDA call, for it may happen at any time (a collected Python object, in the middle of a capture). So those
+// that were left become idle together: a new handle that finds no idle one, but four of them, waits for the device.
 constexpr size_t SCRATCH_PART = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
-constexpr int SCRATCH_KEEP = 16;     // idle ones per device; the rest are released at that time
+constexpr size_t SCRATCH_BYTES = SCRATCH_PART + (PA_MAX_CTAS * sizeof(int) + 255) / 256 * 256;
+constexpr int SCRATCH_KEEP = 16;     // idle ones per device; blocks of four beyond them are released after that wait
 static std::mutex g_scratch_mu;
-static struct { Scratch *idle, *left; } g_scratch[16];
+static struct { Scratch *idle, *left; int n_left; } g_scratch[16];
 
+static Scratch* scratch_pop(int device) {               // an idle one, or null; the lock is held
+  Scratch* s = g_scratch[device].idle;
+  if (s) {
+    g_scratch[device].idle = s->next;
+    s->users = 1;
+  }
+  return s;
+}
 static cudaError_t scratch_take(int device, Scratch*& out) {
-  Scratch* left;
+  auto& kept = g_scratch[device];
+  Scratch* left = nullptr;
   {
     std::lock_guard<std::mutex> lk(g_scratch_mu);
-    auto& kept = g_scratch[device];
-    if ((out = kept.idle)) {
-      kept.idle = out->next;
-      out->users = 1;
-      return cudaSuccess;
+    if ((out = scratch_pop(device))) return cudaSuccess;
+    if (kept.n_left >= SCRATCH_BLOCK) {
+      left = kept.left;
+      kept.left = nullptr;
+      kept.n_left = 0;
     }
-    left = kept.left;
-    kept.left = nullptr;
   }
   if (left) {
     const cudaError_t e = cudaDeviceSynchronize();      // no launch uses these any more
-    Scratch* rest = nullptr;
+    ScratchBlock* unused = nullptr;
     {
       std::lock_guard<std::mutex> lk(g_scratch_mu);
-      auto& kept = g_scratch[device];
       int n = 0;
-      for (Scratch* s = kept.idle; s; s = s->next) ++n;
-      if (e == cudaSuccess) {
-        out = left;
-        left = left->next;
-        out->users = 1;
-      }
-      while (left) {
-        Scratch* s = left;
+      for (Scratch* s = left; s; s = left) {
         left = s->next;
-        Scratch*& list = e != cudaSuccess ? kept.left : n++ < SCRATCH_KEEP ? kept.idle : rest;
+        Scratch*& list = e == cudaSuccess ? kept.idle : kept.left;
+        if (e != cudaSuccess) ++kept.n_left;
         s->next = list;
         list = s;
       }
+      if (e != cudaSuccess) return e;
+      for (Scratch* s = kept.idle; s; s = s->next, ++n) s->block->idle = 0;
+      for (Scratch* s = kept.idle; s; s = s->next) ++s->block->idle;
+      for (Scratch** at = &kept.idle; *at;) {           // whole blocks leave the list
+        ScratchBlock* b = (*at)->block;
+        if (b->idle != SCRATCH_BLOCK || (!b->released && n - SCRATCH_BLOCK < SCRATCH_KEEP)) {
+          at = &(*at)->next;
+          continue;
+        }
+        if (!b->released) {
+          b->released = true;
+          b->next = unused;
+          unused = b;
+          n -= SCRATCH_BLOCK;
+        }
+        *at = (*at)->next;
+      }
+      out = scratch_pop(device);
     }
-    while (rest) {
-      Scratch* s = rest;
-      rest = s->next;
-      cudaFree(s->s.part);
-      delete s;
+    while (unused) {
+      ScratchBlock* b = unused;
+      unused = b->next;
+      cudaFree(b->p);
+      delete b;
     }
+    return cudaSuccess;
+  }
+  ScratchBlock* b = new (std::nothrow) ScratchBlock;
+  if (!b) return cudaErrorMemoryAllocation;
+  cudaError_t e = cudaMalloc(&b->p, SCRATCH_BLOCK * SCRATCH_BYTES);
+  for (int i = 0; e == cudaSuccess && i < SCRATCH_BLOCK; ++i) {
+    char* p = static_cast<char*>(b->p) + i * SCRATCH_BYTES;
+    b->s[i].s.part = reinterpret_cast<float*>(p);
+    b->s[i].s.ticket = reinterpret_cast<int*>(p + SCRATCH_PART);
+    b->s[i].device = device;
+    b->s[i].block = b;
+    e = cudaMemset(b->s[i].s.ticket, 0, PA_MAX_CTAS * sizeof(int));
+  }
+  if (e == cudaSuccess) e = cudaStreamSynchronize(0);   // the first call may be on a stream that does not wait for this one
+  if (e != cudaSuccess) {
+    cudaFree(b->p);
+    delete b;
     return e;
   }
-  if (!(out = new (std::nothrow) Scratch)) return cudaErrorMemoryAllocation;
-  void* p = nullptr;
-  cudaError_t e = cudaMalloc(&p, SCRATCH_PART + PA_MAX_CTAS * sizeof(int));
-  if (e == cudaSuccess) {
-    out->device = device;
-    out->s.part = static_cast<float*>(p);
-    out->s.ticket = reinterpret_cast<int*>(static_cast<char*>(p) + SCRATCH_PART);
-    e = cudaMemset(out->s.ticket, 0, PA_MAX_CTAS * sizeof(int));
-    if (e == cudaSuccess) e = cudaStreamSynchronize(0);   // the first call may be on a stream that does not wait for this one
+  std::lock_guard<std::mutex> lk(g_scratch_mu);
+  for (int i = SCRATCH_BLOCK - 1; i >= 0; --i) {
+    b->s[i].next = kept.idle;
+    kept.idle = &b->s[i];
   }
-  if (e != cudaSuccess) {
-    cudaFree(p);
-    delete out;
-    out = nullptr;
-  }
-  return e;
+  out = scratch_pop(device);
+  return cudaSuccess;
 }
 static void scratch_leave(Scratch* s) {
   if (--s->users) return;
   std::lock_guard<std::mutex> lk(g_scratch_mu);
-  s->next = g_scratch[s->device].left;
-  g_scratch[s->device].left = s;
+  auto& kept = g_scratch[s->device];
+  s->next = kept.left;
+  kept.left = s;
+  ++kept.n_left;
 }
 // A graph under capture on `stream` uses the scratch for as long as the graph, or what was instantiated from it, lives.
 static cudaError_t scratch_hold(Scratch* s, cudaStream_t stream) {
