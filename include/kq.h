@@ -313,7 +313,10 @@ int kq_page_append(kq_pages* c, const kq_append_args* a, void* stream);
 
 /* Attention of one token of each of n sequences over its cached positions t in [0, len[i]) (window > 0:
  * the last `window` of them): out[i][h] = sum_t softmax_t(scale q[i][h] . K[t][g]) V[t][g], with
- * g = h / (n_heads / n_kv_heads), sums and softmax in 32 bits. No position: zeros. The splits of a
+ * g = h / (n_heads / n_kv_heads). Sums and the softmax's statistics are held in 32 bits; what is multiplied are 16-bit terms:
+ * fp32 queries (and fp16 ones on a bf16 cache) in 22 bits on fp16 and e4m3 caches, 24 on bf16 ones, other 16-bit queries as they
+ * are; the softmax's weights in 22 or 24 bits, in 16 for bf16 queries on a bf16 cache. On fp16 and e4m3 caches a query element
+ * below 2^-33 of its head's largest counts as 0, and of 16-bit queries one below 2^-24 loses bits. No position: zeros. The splits of a
  * long sequence are joined in a fixed order, so equal calls give equal bits. Positions outside the
  * range are never read; inside it, an infinite V gives NaN (the weights are multiplied in two parts).
  * Flagged: a table row out of range (zeros), len[i] past the table (cut there), a page id outside
@@ -341,7 +344,7 @@ int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream);
  *   z = -infinity where the row's mask (bit id % 32 of word id / 32) is 0
  * rounded once to `type`. best[i] = the lowest id of the largest output, -1 if all are -infinity or NaN.
  * out may be the logits themselves. Every rule may be absent (null). Ids outside [0, vocab) in a
- * history or a list are ignored (padding). mask_row[i]: row of the mask array, -1: no mask; null: row i.
+ * history or a list are ignored (padding). Lists of up to some hundred biases a row cost little; of thousands, their length squared. mask_row[i]: row of the mask array, -1: no mask; null: row i.
  * Flagged: a mask row out of range (the row then allows nothing). */
 #define KQ_RULES_MAX_VOCAB 393216
 typedef struct {

@@ -108,7 +108,7 @@ struct RlCount<true> {
 // Positions count from the 16-byte boundary at or below the row's start (u = id + shift), so a row whose input and
 // output lie alike moves in 16-byte groups wherever it starts, the groups over its ends element by
 // element; where they lie differently (an odd vocabulary into a padded output) the whole row does.
-// Measured: 128 fp32 rows of 151936 with histories of up to 4096 tokens, 300 biases and masks 48.9 us (3.2
+// Measured: 128 fp32 rows of 151936 with histories of up to 4096 tokens, 300 biases and masks 49.4 us (3.2
 // TB/s read and written; the copy rate would take 23.8: two waves of CTAs, each counting before it
 // streams); in the stream 124, one CTA per row 240, clusters of 16 with the logits held meanwhile 109
 // to 119 (a cluster waits until 16 slots of one GPC are free). One row 6.9 us.

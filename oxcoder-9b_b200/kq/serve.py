@@ -131,7 +131,8 @@ class PagedCache(object):
     or e4m3 (any strides with dense rows on 16-byte boundaries: a transposed view of
     [n_pages, page, n_kv_heads, head_dim] will do). k_scale, v_scale (e4m3 only): fp32 [n_kv_heads], a stored
     x stands for x * scale. The tensors stay the caller's and are kept alive by this object. Calls on
-    one cache that overlap in time on different streams race: use one PagedCache for each stream."""
+    one cache that overlap in time on different streams race: use one PagedCache for each stream. It may
+    be closed or collected at any time; a graph that captured its calls needs the tensors alone."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         lib, check, error = _bind()
