@@ -344,7 +344,7 @@ int kq_page_attend(kq_pages* c, const kq_attend_args* a, void* stream);
  *   z = -infinity where the row's mask (bit id % 32 of word id / 32) is 0
  * rounded once to `type`. best[i] = the lowest id of the largest output, -1 if all are -infinity or NaN.
  * out may be the logits themselves. Every rule may be absent (null). Ids outside [0, vocab) in a
- * history or a list are ignored (padding). Lists of up to some hundred biases a row cost little; of thousands, their length squared. mask_row[i]: row of the mask array, -1: no mask; null: row i.
+ * history or a list are ignored (padding). mask_row[i]: row of the mask array, -1: no mask; null: row i.
  * Flagged: a mask row out of range (the row then allows nothing). */
 #define KQ_RULES_MAX_VOCAB 393216
 typedef struct {

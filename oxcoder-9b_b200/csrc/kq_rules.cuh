@@ -79,7 +79,8 @@ constexpr int RL_CLUSTER = 16;       // CTAs of a row at most
 constexpr int RL_BYTES = 76 * 1024;  // of counts a CTA holds at most if it may: two CTAs per SM
 constexpr int RL_BATCH = 2;          // 16-byte groups of logits a thread requests ahead (4 or 6: more code, slower)
 constexpr int RL_TOUCH = 2048;       // touched ids a CTA lists; where there are more it goes through its counts
-constexpr int RL_LIST = 512;         // bias entries of a CTA's ids that it keeps; a longer list is searched where it stands
+constexpr int RL_LIST = 512;         // bias entries of a CTA's ids that it keeps; a longer list is read again, an entry per thread
+static_assert(RL_LIST == RL_THREADS, "the kept entries' places serve as a thread's slot each");
 constexpr int RL_LOCAL = 16384;      // histories up to here are scanned by every CTA of the row
 
 // Counts of a CTA's ids in shared memory: 16 bits an id, or 32 where histories may be longer. Beside the
@@ -338,40 +339,62 @@ __global__ void __launch_bounds__(RL_THREADS, 2) k_logit_rules(const __grid_cons
 
   if (counted) {
     __syncthreads();                                      // the stream has written the touched ids too
-    const int entries = s_entries;
-    // v: the id's logit (in place: the value itself, or masked and about to be again)
-    auto apply = [&](int h, uint32_t c, float v, uint32_t word) {
+    const int entries = s_entries, kept = entries > RL_LIST ? 0 : entries;
+    // v: the id's logit (in place: the value itself, or masked and about to be again), b: its bias
+    auto apply = [&](int h, uint32_t c, float v, float b, uint32_t word) {
       if (c & ~K::BIASED) v = rl_penalise(v, (c & K::MOST) | ((c & K::PROMPT) ? 0x80000000u : 0u), rep, freq, pres);
-      if (c & K::BIASED) {                                // the last entry of the list with this id
-        int top = -1;
-        float b = 0.f;
-        if (entries <= RL_LIST) {
-          for (int e = 0; e < entries; ++e)
-            if (s_id[e] == h && s_entry[e] > top) {
-              top = s_entry[e];
-              b = s_bias[e];
-            }
-        } else {
-          for (top = P.n_bias - 1; bias_id[top] != h;) --top;
-          b = P.bias[i * P.bias_ld + top];
-        }
-        v = __fadd_rn(v, b);
-      }
+      if (c & K::BIASED) v = __fadd_rn(v, b);
       if (none || !((word >> (h & 31)) & 1u)) v = -INFINITY;
       const T r = rl_put<T>(v);
       out[h] = r;
       const float f = rl_get<T>(r);
       if (f > -INFINITY) better(f, h);
     };
+    auto bias_of = [&](int h, uint32_t c) {               // the last entry of the list with this id
+      int last = -1;
+      float b = 0.f;
+      if (c & K::BIASED)
+        for (int e = 0; e < kept; ++e)
+          if (s_id[e] == h && s_entry[e] > last) {
+            last = s_entry[e];
+            b = s_bias[e];
+          }
+      return b;
+    };
+    if (entries > RL_LIST) {
+      // more entries than are kept: the list from its end, a thread an entry. Of the entries whose ids share a slot
+      // the last one stands and its id is done; another id of the slot is left for the next turn. (128 rows of 151936
+      // with 300 / 2000 / 10000 / 151936 entries 40 / 76 / 168 / 1760 us; a search of the list for each id took 348 us for
+      // 2000 and 66 ms for 10000. Short lists pay up to 0.25 us for the larger kernel.)
+      for (int j1 = P.n_bias - 1; j1 >= 0; j1 -= RL_THREADS) {
+        const int j = j1 - tid, h = j >= 0 ? bias_id[j] : -1, at = mine(h) ? local(h + shift) : -1;
+        bool open = at >= 0 && (cnt[at] & K::BIASED);
+        while (__syncthreads_or(open)) {
+          s_entry[tid] = -1;
+          __syncthreads();
+          if (open) atomicMax(&s_entry[h & (RL_LIST - 1)], j);
+          __syncthreads();
+          if (open && s_entry[h & (RL_LIST - 1)] == j) {
+            apply(h, cnt[at], rl_get<T>(in[h]), P.bias[i * P.bias_ld + j], mask_of(h));
+            cnt[at] = 0;
+          }
+          __syncthreads();
+          open = open && (cnt[at] & K::BIASED);
+        }
+      }
+    }
     if (!apart && s_n <= RL_TOUCH) {
       for (int e = tid; e < s_n; e += RL_THREADS) {
         const int h = s_touched[e];
-        apply(h, cnt[local(h + shift)], rl_get<T>(in[h]), mask_of(h));
+        const uint32_t c = cnt[local(h + shift)], word = mask_of(h);
+        const float v = rl_get<T>(in[h]);                 // on its way while the list is searched
+        if (c) apply(h, c, v, bias_of(h, c), word);
       }
     } else {
       for (int at = tid; at < span; at += RL_THREADS) {
         const int h = place(at / STEP) + (at & (STEP - 1)) - shift;
-        if (cnt[at]) apply(h, cnt[at], rl_get<T>(in[h]), mask_of(h));
+        const uint32_t c = cnt[at];
+        if (c) apply(h, c, rl_get<T>(in[h]), bias_of(h, c), mask_of(h));
       }
     }
   }
