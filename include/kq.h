@@ -280,7 +280,7 @@ typedef struct kq_pages kq_pages;       /* opaque: the description and the atten
  * calls on the handle still run, or during a stream capture, and a graph that captured calls may be replayed after it (the
  * graph keeps the scratch; the tensors are the caller's to keep). Replays on one stream and calls or replays that use the
  * same handle on another race like calls do. Scratches (10 MB each)
- * come in blocks of four and are kept for the next handles; once in about four handles kq_pages_create waits for the device, so
+ * come in blocks of four and are kept for the next handles; once in a few handles kq_pages_create waits for the device, so
  * that those of freed handles are used again, and releases idle blocks beyond four. NULL on failure, see kq_error. */
 kq_pages* kq_pages_create(const kq_page_desc* d, int device);
 void kq_pages_free(kq_pages* c);

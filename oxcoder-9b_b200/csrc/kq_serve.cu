@@ -132,7 +132,7 @@ static int pages_check(const kq_page_desc* d) {
 // drops handles while it runs, and an allocation costs some milliseconds. Between launches a scratch's tickets are
 // zero, so it can be handed on as it is. Launches may still use a scratch when its last user leaves, and leaving
 // makes no CUDA call, for it may happen at any time (a collected Python object, in the middle of a capture). So those
-// that were left become idle together: a new handle that finds no idle one, but four of them, waits for the device.
+// that were left become idle together: a new handle that finds no idle one, but two of them, waits for the device.
 constexpr size_t SCRATCH_PART = (size_t)2 * PA_MAX_CTAS * PA_MAX_HEADS * PA_PLD * sizeof(float);
 constexpr size_t SCRATCH_BYTES = SCRATCH_PART + (PA_MAX_CTAS * sizeof(int) + 255) / 256 * 256;
 constexpr int SCRATCH_KEEP = 16;     // idle ones per device; blocks of four beyond them are released after that wait
@@ -153,7 +153,7 @@ static cudaError_t scratch_take(int device, Scratch*& out) {
   {
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     if ((out = scratch_pop(device))) return cudaSuccess;
-    if (kept.n_left >= SCRATCH_BLOCK) {
+    if (kept.n_left >= 2) {
       left = kept.left;
       kept.left = nullptr;
       kept.n_left = 0;
